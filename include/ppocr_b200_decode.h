@@ -1,0 +1,119 @@
+// Operators of an autoregressive text decoder (libppocr_b200.so): a paged
+// key/value cache held in 4 bits, the attention that reads it, and token
+// sampling. Together with ppocr_b200_gemm_epilogue and ppocr_b200_layernorm
+// they make up a decoder's step over the recognizer's hidden states.
+//
+// Return 0 on success, -1 on failure (message: ppocr_b200_last_error()).
+// All pointers are device memory unless stated; every call is asynchronous on
+// `stream`. What a kernel finds wrong in device data (a page id outside the
+// pool, a length above the table's capacity, more new tokens than max_new)
+// is never followed out of bounds; it sets the code that
+// ppocr_b200_device_error() returns: 61 page id, 62 length or offsets.
+#pragma once
+#include <cuda_runtime_api.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+// Element types of queries, keys, values and outputs (and of logits).
+enum { PPOCR_B200_F16 = 0, PPOCR_B200_BF16 = 1, PPOCR_B200_F32 = 2 };
+
+// A cache of `pages` pages of page_size tokens (16, 32, 64 or 128) for
+// kv_heads heads of head_dim channels (32, 64 or 128), in a pool of
+// pages * kv_heads * ppocr_b200_kv4_block_bytes() bytes, 16-byte aligned.
+// One (page, head) block holds, with G = head_dim / 32 groups per token:
+//   key codes    [page_size][head_dim / 2]  two channels a byte, the even one
+//                                           in the low nibble
+//   value codes  [page_size][head_dim / 2]
+//   key groups   [page_size][G] (scale, minimum), 16 bits each, in `type`
+//   value groups [page_size][G] (scale, minimum)
+// A code c in 0..15 stands for minimum + scale * c.
+typedef struct PpocrKv4Cache {
+  void *pool;
+  long long pages;
+  int page_size, kv_heads, head_dim;
+  int type; // PPOCR_B200_F16 or PPOCR_B200_BF16
+} PpocrKv4Cache;
+
+// Bytes of one (page, head) block; 0 for a geometry that is not supported.
+size_t ppocr_b200_kv4_block_bytes(int page_size, int head_dim);
+
+// Where the tokens of a call sit, the same for the three calls below:
+//   table   int32 [batch][width]  page ids of each sequence's positions
+//   lengths int32 [batch]         tokens of each sequence, the new ones among
+//                                 them (the new ones are its last)
+//   starts  int32 [batch + 1]     sequence b's new tokens are rows starts[b] ..
+//                                 starts[b + 1] - 1 of the packed arrays; null:
+//                                 max_new each (tokens = batch * max_new)
+//   tokens  rows of the packed arrays; max_new: no sequence has more new ones
+// A new token whose position would be negative (more new tokens than the
+// length) is not written, reads back as zero and sees no key.
+
+// Quantises the new tokens' keys and values into the cache. k and v are
+// [tokens][kv_heads][head_dim] of the cache's type with rows k_stride and
+// v_stride elements apart (multiples of 8; 16-byte aligned), so slices of a
+// fused projection need no copy. Per group of 32 channels: minimum = min x,
+// scale = round16((max x - min x) / 15), code = clamp(rint((x - minimum) *
+// (1 / scale)), 0, 15), computed in fp32. NaN is stored as 0; values beyond
+// +-65000 (fp16) or +-2^126 (bf16) saturate there.
+int ppocr_b200_kv4_append(const PpocrKv4Cache *cache, const void *k,
+                          long long k_stride, const void *v,
+                          long long v_stride, const int *table, int width,
+                          const int *lengths, const int *starts, int batch,
+                          int tokens, int max_new, cudaStream_t stream);
+
+// The values that the cache holds for those tokens: k and v
+// [tokens][kv_heads][head_dim], contiguous, 16-byte aligned.
+int ppocr_b200_kv4_read(const PpocrKv4Cache *cache, void *k, void *v,
+                        const int *table, int width, const int *lengths,
+                        const int *starts, int batch, int tokens, int max_new,
+                        cudaStream_t stream);
+
+// Attention of the new tokens over the cache (which holds their own keys and
+// values already): out[i][h] = sum_t softmax_t(scale * q[i][h] . k[t]) v[t]
+// with the keys and values of head h / (heads / kv_heads). The token at
+// position p sees position t when t <= p and, with window > 0, either
+// t > p - window or t < sinks. A token that sees nothing gets zeros. q rows
+// are q_stride elements apart (heads contiguous), out [tokens][heads]
+// [head_dim] contiguous; both of the cache's type and 16-byte aligned.
+// Softmax statistics and sums are fp32. workspace: device memory of
+// ppocr_b200_kv4_workspace_bytes() bytes, 256-byte aligned, zeroed once
+// before its first use (every call leaves it ready for the next); calls that
+// may overlap on the GPU need one each.
+size_t ppocr_b200_kv4_workspace_bytes(void);
+int ppocr_b200_kv4_attention(const PpocrKv4Cache *cache, const void *q,
+                             long long q_stride, void *out, int heads,
+                             float scale, int window, int sinks,
+                             const int *table, int width, const int *lengths,
+                             const int *starts, int batch, int tokens,
+                             int max_new, void *workspace,
+                             cudaStream_t stream);
+
+// One token per row of logits [rows][vocab] (type F16, BF16 or F32; rows
+// `stride` elements apart). Per row, each parameter array may be null (off):
+//   temperature  T > 0 divides the logits; anything else takes the largest
+//   top_k        > 0: only the k largest logits
+//   top_p        < 1: of those, the fewest largest whose probability reaches p
+//   min_p        > 0: none less probable than min_p times the most probable
+// Larger logits come first, equal ones by index; the first one always stays.
+// uniform[row] in [0, 1) picks from what stays, in index order: the first id
+// whose running share exceeds it. NaN counts as -inf.
+// Probabilities are whole numbers, floor(exp(-(max - x) / T) * 2^32), and top_p
+// and uniform are taken in steps of 2^-24: sums do not depend on their order,
+// so the same inputs give the same ids on any split of the work.
+//   ids[row]   the token; -1 where every logit is -inf
+//   prob[row]  its probability at T (at 1 where T is not above 0) before
+//              top_k, top_p and min_p
+//   kept[row]  how many tokens stayed
+int ppocr_b200_sample(const void *logits, int type, long long stride, int rows,
+                      int vocab, const float *temperature, const int *top_k,
+                      const float *top_p, const float *min_p,
+                      const float *uniform, int *ids, float *prob, int *kept,
+                      cudaStream_t stream);
+
+#ifdef __cplusplus
+}
+#endif

@@ -1,0 +1,113 @@
+"""Plain restatements of the text decoder's operators
+(include/ppocr_b200_decode.h): the 4-bit cache's format, the attention over it
+and token sampling, in 64 bits where values are computed. CPU only."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+GROUP = 32
+LIMIT = {torch.float16: 65000.0, torch.bfloat16: 2.0 ** 126}
+
+
+def block_bytes(page_size: int, dim: int) -> int:
+    return page_size * (dim + dim // GROUP * 8)
+
+
+def quantise(x: torch.Tensor):
+    """Codes (uint8), scales and minimums of [..., dim] 16-bit values; the
+    arithmetic is fp32 by definition."""
+    t = x.dtype
+    y = torch.where(torch.isnan(x), torch.zeros_like(x), x).float().clamp(-LIMIT[t], LIMIT[t])
+    y = y.unflatten(-1, (-1, GROUP))
+    low = y.amin(-1).to(t)
+    scale = ((y.amax(-1) - low.float()) / 15).to(t)
+    s = scale.float()[..., None]
+    inv = torch.where(s > 1e-30, 1 / s, torch.zeros_like(s))
+    codes = torch.round(((y - low.float()[..., None]) * inv).clamp(0, 15))
+    return codes.flatten(-2).to(torch.uint8), scale, low
+
+
+def restore(codes, scale, low, dtype=torch.float64):
+    c = codes.to(dtype).unflatten(-1, (-1, GROUP))
+    return (low.to(dtype)[..., None] + scale.to(dtype)[..., None] * c).flatten(-2)
+
+
+def views(pool: torch.Tensor, page_size: int, dim: int, t: torch.dtype):
+    """(key codes, value codes, key groups, value groups) of pool
+    [pages, heads, block], writable views by page, head and slot."""
+    n, m = page_size * dim // 2, page_size * (dim // GROUP) * 4
+    out = [pool[..., a:a + n].unflatten(-1, (page_size, dim // 2)) for a in (0, n)]
+    out += [pool[..., a:a + m].view(t).unflatten(-1, (page_size, dim // GROUP, 2)) for a in (2 * n, 2 * n + m)]
+    return out
+
+
+def write(pool, page_size, dim, t, x, which, page, slot):
+    """Stores x [heads, dim] as the key (which 0) or value (1) of one token."""
+    v = views(pool, page_size, dim, t)
+    codes, scale, low = quantise(x)
+    v[which][page, :, slot] = codes[:, 0::2] | (codes[:, 1::2] << 4)
+    v[2 + which][page, :, slot] = torch.stack([scale, low], -1)
+
+
+def held(pool, page_size, dim, t, table_row, length, which):
+    """The keys (0) or values (1) [length, heads, dim] of a sequence, fp64."""
+    v = views(pool, page_size, dim, t)
+    pos = torch.arange(length)
+    page = table_row.long()[pos // page_size]
+    byte = v[which][page, :, pos % page_size]
+    codes = torch.stack([byte & 15, byte >> 4], -1).flatten(-2)
+    g = v[2 + which][page, :, pos % page_size]
+    return restore(codes, g[..., 0], g[..., 1])
+
+
+def attention(q, k, v, first_pos, scale, window=0, sinks=0):
+    """q [n, heads, dim] at positions first_pos.., k and v [len, kv, dim]
+    (fp64): (out, sum of p |v|, largest scale * sum |q k| of a visible key),
+    each fp64; rows that see nothing are zero."""
+    n, heads, dim = q.shape
+    out = torch.zeros(n, heads, dim, dtype=torch.float64)
+    mag = torch.zeros_like(out)
+    most = torch.zeros(n, heads, dtype=torch.float64)
+    if k.shape[0] == 0:
+        return out, mag, most
+    group = heads // k.shape[1]
+    key = torch.arange(k.shape[0])
+    for i in range(n):
+        p = first_pos + i
+        see = key <= p
+        if window > 0:
+            see &= (key > p - window) | (key < sinks)
+        if not see.any():
+            continue
+        for h in range(heads):
+            kk, vv = k[see, h // group], v[see, h // group]
+            x = q[i, h].double()
+            w = torch.softmax(scale * (kk @ x), 0)
+            out[i, h] = w @ vv
+            mag[i, h] = w @ vv.abs()
+            most[i, h] = abs(scale) * (kk.abs() @ x.abs()).max()
+    return out, mag, most
+
+
+def sample_row(x, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The distribution that one row's token is drawn from, in fp64: (order
+    of the ids, their probabilities at the temperature, the number that
+    stay). x: 1-D logits."""
+    x = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x).double()
+    if not temperature > 0:
+        temperature, top_k = 1.0, 1
+    top = x.max()
+    d = torch.where(x == top, torch.zeros_like(x), (top - x) / temperature)
+    p = torch.exp(-d)
+    p = p / p.sum()
+    order = torch.sort(x, descending=True, stable=True).indices
+    ps = p[order]
+    n = min(top_k, len(ps)) if top_k > 0 else len(ps)
+    if top_p < 1:
+        before = ps[:n].cumsum(0) - ps[:n]
+        n = max(1, int((before < top_p * ps[:n].sum()).sum()))
+    n = max(1, min(n, int((ps >= min_p * ps[0]).sum())))
+    return order, ps, n

@@ -1,6 +1,8 @@
 // extern "C" boundary of libppocr_b200.so: the head API
-// (include/ppocr_b200_head.h) and the operator-level entry points
-// (include/ppocr_b200_ops.h). Thin argument checks + kernels.h launchers.
+// (include/ppocr_b200_head.h), the operator-level entry points
+// (include/ppocr_b200_ops.h) and the text decoder's operators
+// (include/ppocr_b200_decode.h). Thin argument checks + kernels.h launchers.
+#include "../../include/ppocr_b200_decode.h"
 #include "../../include/ppocr_b200_head.h"
 #include "../../include/ppocr_b200_ops.h"
 #include "../../include/ppocr_b200_preprocess.h"
@@ -63,6 +65,52 @@ void *stream_workspace(size_t bytes, cudaStream_t stream) {
 }
 
 size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+bool aligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Checks what the three cache calls share. Returns null, or what is wrong.
+const char *kv4_arguments(const PpocrKv4Cache *cache, const int *table, int width, const int *lengths,
+                          const int *starts, int batch, int tokens, int max_new, Kv4Cache &c, Kv4Tokens &t) {
+  if (!cache || !cache->pool || !aligned(cache->pool, 16))
+    return "cache pool missing or not 16-byte aligned";
+  if (cache->type != PPOCR_B200_F16 && cache->type != PPOCR_B200_BF16)
+    return "cache type must be f16 or bf16";
+  if (!ppocr_b200_kv4_block_bytes(cache->page_size, cache->head_dim))
+    return "page size must be 16, 32, 64 or 128 and head_dim 32, 64 or 128";
+  if (cache->kv_heads <= 0 || cache->pages <= 0 || cache->pages > ((1ll << 31) - 1) / cache->kv_heads)
+    return "pages and kv_heads must be positive, pages * kv_heads below 2^31";
+  if (batch < 0 || batch > 65535 || tokens < 0 || max_new < 0)
+    return "batch (at most 65535), tokens and max_new must not be negative";
+  if (!table || !lengths || width <= 0 || width >= (1 << 30) / cache->page_size)
+    return "table or lengths missing, or table width out of range";
+  if (!starts && static_cast<long long>(batch) * max_new != tokens)
+    return "without starts, tokens must be batch * max_new";
+  c.pool = static_cast<uint8_t *>(cache->pool);
+  c.pages = cache->pages;
+  c.page_size = cache->page_size;
+  c.kv_heads = cache->kv_heads;
+  c.head_dim = cache->head_dim;
+  c.bf16 = cache->type == PPOCR_B200_BF16;
+  t.table = table;
+  t.lengths = lengths;
+  t.starts = starts;
+  t.width = width;
+  t.batch = batch;
+  t.tokens = tokens;
+  t.max_new = max_new;
+  t.pages = static_cast<int>(cache->pages);
+  while ((1 << t.page_shift) < cache->page_size)
+    ++t.page_shift;
+  t.err = device_error_word();
+  return nullptr;
+}
+// New tokens of one sequence, in 8-channel chunks of all key heads, are
+// counted in 32 bits.
+const char *kv4_row_arguments(const PpocrKv4Cache *cache, int max_new) {
+  return static_cast<long long>(max_new) * cache->kv_heads * (cache->head_dim / 8) >= (1ll << 31)
+             ? "max_new * kv_heads * head_dim is too large"
+             : nullptr;
+}
 } // namespace
 
 void pb2::set_last_error(const std::string &message) { g_error = message; }
@@ -689,6 +737,118 @@ int ppocr_b200_f16_to_f32(const void *x, float *y, size_t n,
   if (!x || !y)
     return fail("invalid conversion arguments");
   return status(half_to_float(H(x), y, n, stream), "f16_to_f32");
+}
+
+size_t ppocr_b200_kv4_block_bytes(int page_size, int head_dim) {
+  if ((page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) ||
+      (head_dim != 32 && head_dim != 64 && head_dim != 128))
+    return 0;
+  return kv4_block_bytes(page_size, head_dim);
+}
+
+int ppocr_b200_kv4_append(const PpocrKv4Cache *cache, const void *k, long long k_stride, const void *v,
+                          long long v_stride, const int *table, int width, const int *lengths, const int *starts,
+                          int batch, int tokens, int max_new, cudaStream_t stream) {
+  g_error.clear();
+  Kv4Cache c;
+  Kv4Tokens t;
+  const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
+  if (!bad)
+    bad = kv4_row_arguments(cache, max_new);
+  if (bad)
+    return fail(std::string("kv4 append: ") + bad);
+  if (batch == 0 || tokens == 0 || max_new == 0)
+    return 0;
+  const long long row = static_cast<long long>(c.kv_heads) * c.head_dim;
+  if (!k || !v || !aligned(k, 16) || !aligned(v, 16) || k_stride < row || v_stride < row || k_stride % 8 ||
+      v_stride % 8)
+    return fail("kv4 append: k and v must be 16-byte aligned, with row strides of at least a row and a multiple of 8");
+  return status(kv4_append(c, t, k, k_stride, v, v_stride, stream), "kv4 append");
+}
+
+int ppocr_b200_kv4_read(const PpocrKv4Cache *cache, void *k, void *v, const int *table, int width,
+                        const int *lengths, const int *starts, int batch, int tokens, int max_new,
+                        cudaStream_t stream) {
+  g_error.clear();
+  Kv4Cache c;
+  Kv4Tokens t;
+  const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
+  if (!bad)
+    bad = kv4_row_arguments(cache, max_new);
+  if (bad)
+    return fail(std::string("kv4 read: ") + bad);
+  if (batch == 0 || tokens == 0 || max_new == 0)
+    return 0;
+  if (!k || !v || !aligned(k, 16) || !aligned(v, 16))
+    return fail("kv4 read: k and v must be 16-byte aligned");
+  return status(kv4_read(c, t, k, v, stream), "kv4 read");
+}
+
+size_t ppocr_b200_kv4_workspace_bytes(void) { return kv4_workspace_bytes(); }
+
+int ppocr_b200_kv4_attention(const PpocrKv4Cache *cache, const void *q, long long q_stride, void *out, int heads,
+                             float scale, int window, int sinks, const int *table, int width, const int *lengths,
+                             const int *starts, int batch, int tokens, int max_new, void *workspace,
+                             cudaStream_t stream) {
+  g_error.clear();
+  Kv4Cache c;
+  Kv4Tokens t;
+  const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
+  if (bad)
+    return fail(std::string("kv4 attention: ") + bad);
+  if (heads <= 0 || heads % c.kv_heads)
+    return fail("kv4 attention: heads must be a multiple of kv_heads");
+  if (static_cast<long long>(max_new) * (heads / c.kv_heads) >= (1ll << 30))
+    return fail("kv4 attention: max_new * heads / kv_heads is too large");
+  if (window < 0 || sinks < 0 || !(scale - scale == 0.f))
+    return fail("kv4 attention: window and sinks must not be negative, scale must be finite");
+  if (batch == 0 || tokens == 0 || max_new == 0)
+    return 0;
+  if (!q || !out || !aligned(q, 16) || !aligned(out, 16) || q_stride % 8 ||
+      q_stride < static_cast<long long>(heads) * c.head_dim)
+    return fail("kv4 attention: q and out must be 16-byte aligned, q's row stride at least a row and a multiple of 8");
+  if (!workspace || !aligned(workspace, 256))
+    return fail("kv4 attention: workspace missing or not 256-byte aligned");
+  Kv4Attention a;
+  a.q = q;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.heads = heads;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale = scale;
+  a.workspace = workspace;
+  return status(kv4_attend_rows(c, t, a, stream), "kv4 attention");
+}
+
+int ppocr_b200_sample(const void *logits, int type, long long stride, int rows, int vocab, const float *temperature,
+                      const int *top_k, const float *top_p, const float *min_p, const float *uniform, int *ids,
+                      float *prob, int *kept, cudaStream_t stream) {
+  g_error.clear();
+  if (type != PPOCR_B200_F16 && type != PPOCR_B200_BF16 && type != PPOCR_B200_F32)
+    return fail("sample: type must be f16, bf16 or f32");
+  // A row's mass is at most vocab * 2^32 and has to fit 63 bits with room.
+  if (rows < 0 || vocab <= 0 || vocab > (1 << 24) || stride < vocab)
+    return fail("sample: rows, vocab (at most 2^24) or stride out of range");
+  if (rows == 0)
+    return 0;
+  const size_t size = type == PPOCR_B200_F32 ? 4 : 2;
+  if (!logits || !aligned(logits, size) || !uniform || !ids || !prob || !kept)
+    return fail("sample: logits, uniform, ids, prob or kept missing or misaligned");
+  SampleArgs a;
+  a.logits = logits;
+  a.stride = stride;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.uniform = uniform;
+  a.ids = ids;
+  a.prob = prob;
+  a.kept = kept;
+  return status(sample_tokens(a, type, stream), "sample");
 }
 
 } // extern "C"

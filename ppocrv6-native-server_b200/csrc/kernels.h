@@ -349,4 +349,55 @@ cudaError_t roi_warp(const uint8_t *src, int src_h, int src_w, long long src_ste
                      int batch, int dst_h, int dst_w, int out_bgr, int fmt,
                      cudaStream_t stream);
 
+// ------------------------------------------------- text decoder (4-bit cache)
+// The cache of include/ppocr_b200_decode.h and the place of a call's tokens.
+struct Kv4Cache {
+  uint8_t *pool = nullptr;
+  long long pages = 0;
+  int page_size = 0, kv_heads = 0, head_dim = 0;
+  bool bf16 = false;
+};
+struct Kv4Tokens {
+  const int *table = nullptr, *lengths = nullptr, *starts = nullptr;
+  int width = 0, batch = 0, tokens = 0, max_new = 0;
+  int page_shift = 0; // log2 of the page size
+  int pages = 0;
+  int *err = nullptr; // the device error word
+};
+// Bytes of one (page, head) block: codes of keys and values, then 4 bytes a
+// group of 32 channels of each.
+constexpr size_t kv4_block_bytes(int page_size, int head_dim) {
+  return static_cast<size_t>(page_size) * (head_dim + head_dim / 32 * 8);
+}
+cudaError_t kv4_append(const Kv4Cache &c, const Kv4Tokens &t, const void *k, long long k_stride, const void *v,
+                       long long v_stride, cudaStream_t stream);
+cudaError_t kv4_read(const Kv4Cache &c, const Kv4Tokens &t, void *k, void *v, cudaStream_t stream);
+// Attention with few query rows per (sequence, key head): the cache is split
+// over the GPU's CTAs and the parts are joined through `workspace`.
+size_t kv4_workspace_bytes();
+struct Kv4Attention {
+  const void *q = nullptr;
+  void *out = nullptr;
+  long long q_stride = 0;
+  int heads = 0, window = 0, sinks = 0;
+  float scale = 0.f;
+  void *workspace = nullptr;
+};
+cudaError_t kv4_attend_rows(const Kv4Cache &c, const Kv4Tokens &t, const Kv4Attention &a, cudaStream_t stream);
+// Token sampling (csrc/sample.cu); the parameters are per row, null = off.
+struct SampleArgs {
+  const void *logits = nullptr;
+  long long stride = 0; // elements between rows
+  int rows = 0, vocab = 0;
+  const float *temperature = nullptr;
+  const int *top_k = nullptr;
+  const float *top_p = nullptr, *min_p = nullptr;
+  const float *uniform = nullptr;
+  int *ids = nullptr;
+  float *prob = nullptr;
+  int *kept = nullptr;
+};
+enum LogitType { LOGIT_F16 = 0, LOGIT_BF16 = 1, LOGIT_F32 = 2 };
+cudaError_t sample_tokens(const SampleArgs &a, int type, cudaStream_t stream);
+
 } // namespace pb2

@@ -1,0 +1,70 @@
+// What the kernels of the 4-bit key/value cache share: its geometry, the
+// place of a call's tokens, and the conversions between codes and values.
+#pragma once
+#include "kernels.h"
+#include "ptx.cuh"
+#include <cuda_bf16.h>
+
+namespace pb2 {
+
+// Codes stored in the device error word.
+constexpr int kErrPage = 61, kErrLength = 62;
+
+__device__ __forceinline__ void kv4_fault(const Kv4Tokens &t, int code) {
+  if (t.err)
+    atomicCAS(t.err, 0, code);
+}
+
+struct Kv4Seq {
+  int first; // row of the first new token in the packed arrays
+  int n;     // new tokens
+  int len;   // tokens in the cache, the new ones included
+};
+// Sequence b, held to what the arrays can take.
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Tokens &t, int b) {
+  Kv4Seq s;
+  int a = t.starts ? t.starts[b] : b * t.max_new;
+  int e = t.starts ? t.starts[b + 1] : a + t.max_new;
+  s.len = t.lengths[b];
+  const int room = t.width << t.page_shift;
+  if (a < 0 || e < a || e > t.tokens || e - a > t.max_new || s.len < 0 || s.len > room)
+    kv4_fault(t, kErrLength);
+  s.first = min(max(a, 0), t.tokens);
+  s.n = min(min(max(e, s.first), t.tokens) - s.first, t.max_new);
+  s.len = min(max(s.len, 0), room);
+  return s;
+}
+// The page of a position (0 for an id outside the pool, which sets the code).
+__device__ __forceinline__ int kv4_page(const Kv4Tokens &t, int b, int pos) {
+  int p = t.table[static_cast<long long>(b) * t.width + (pos >> t.page_shift)];
+  if (p < 0 || p >= t.pages) {
+    kv4_fault(t, kErrPage);
+    p = 0;
+  }
+  return p;
+}
+
+// 16-bit values by type: F16 or BF16.
+template <bool BF16> __device__ __forceinline__ float kv4_lo(uint32_t w) {
+  if constexpr (BF16)
+    return __uint_as_float(w << 16);
+  else
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(w & 0xFFFFu)));
+}
+template <bool BF16> __device__ __forceinline__ float kv4_hi(uint32_t w) {
+  if constexpr (BF16)
+    return __uint_as_float(w & 0xFFFF0000u);
+  else
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(w >> 16)));
+}
+template <bool BF16> __device__ __forceinline__ uint32_t kv4_pack(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+}
+
+} // namespace pb2

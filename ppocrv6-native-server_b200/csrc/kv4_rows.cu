@@ -1,0 +1,859 @@
+// Attention over the 4-bit cache for few query rows per (sequence, key head):
+// single tokens, a few speculated tokens, short remainders.
+//
+// The work is the reading of the cache (D/2 + D/8 bytes per key and as many
+// per value, 160 together at D = 128), so it is split over key tiles, not
+// over heads: the tiles of all (sequence, row group, key head) units are laid
+// end to end and every CTA takes an equal run of them, whatever the lengths
+// (each CTA scans the lengths itself). A unit that several CTAs share is
+// joined by the last of them to finish, from fp32 parts (m, l, O) in the
+// workspace, in the order of the CTAs.
+//
+// A CTA is four consumer warps and a producer warp that keeps a ring of
+// 128-key stages filled: one tensor copy (keys' and values' codes, swizzled
+// on the way so that the reads below are free of bank conflicts) and one bulk
+// copy (the groups' parameters) per page. Each warp takes 32 keys of a tile,
+// in two slices of 16, with its own running maximum:
+//  * S^T = K q^T by m16n8k16: keys are the 16 rows, 8 query rows the columns.
+//    The keys' codes are fed as they lie: a nibble masked out of its 16-bit
+//    half is the fp16 subnormal c 2^-24 (or 16 c 2^-24, with q / 16), which
+//    the tensor cores multiply exactly, so keys are not rounded at all. Query
+//    rows are scaled by a power of two to just below 2^14 first (exact, and
+//    bf16 queries fit fp16 this way). A group's dot product becomes
+//    scale * (q . c) + minimum * sum(q) in fp32.
+//  * P^T in 16 bits (p is at most 2^8, see below; rounding it costs 2^-12 or
+//    2^-9 relative per term, the precision of the output's own type);
+//    movmatrix turns it into the second product's operand.
+//  * O^T = V^T P^T with the values restored to 16 bits: minimum + scale * c
+//    rounded once, again the precision of the cache's type.
+// The running maximum is only raised when a score passes it by more than 8
+// (in powers of two): until then p stays below 2^8 and nothing is rescaled.
+//
+// Keys past a sequence's length are never used: their scores are replaced
+// (not multiplied) and their values' parameters zeroed, so a page may hold
+// anything there.
+#include "kv4.cuh"
+#include <algorithm>
+
+namespace pb2 {
+namespace {
+
+constexpr int kTile = 128;    // keys per stage
+constexpr int kWarps = 4;     // consumers, 32 keys of a tile each
+constexpr int kRowsThreads = 32 * (kWarps + 1);
+constexpr int kMinTiles = 2;  // tiles a CTA takes at least
+constexpr int kMaxEntries = 2048; // (sequence, row group) entries per launch
+constexpr int kMaxUnits = 1 << 16; // counters in the workspace
+constexpr int kMaxCtas = 148 * 3;
+constexpr int kPartFloats = 16 * (128 + 2);
+constexpr int kErrRowsWait = 42;
+
+struct RowsArgs {
+  Kv4Tokens t;
+  const uint8_t *pool;
+  const uint16_t *q;
+  uint16_t *out;
+  long long q_stride;
+  int heads, kv_heads, group;
+  int window, sinks;
+  float scale_log2; // softmax scale * log2(e)
+  int b0, nb, rg0, nrg; // this launch's sequences and row groups
+  int *counters;
+  float *parts;
+  FastDiv group_div;
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint2 lds_v2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void consumer_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// The key tiles that a row group sees: [0, sink) and [lo, hi).
+struct TileSpan {
+  int sink, lo, n;
+  __device__ __forceinline__ int tile(int j) const { return j < sink ? j : j - sink + lo; }
+};
+struct Group {
+  Kv4Seq s;
+  int row0, rows;       // first row; rows of the group that exist
+  int pos_lo, pos_hi;   // positions of its first and last row
+};
+template <int ROWS> __device__ __forceinline__ Group group_of(const RowsArgs &g, int b, int rg) {
+  Group x;
+  x.s = kv4_seq(g.t, b);
+  x.row0 = rg * ROWS;
+  x.rows = min(max(x.s.n * g.group - x.row0, 0), ROWS);
+  const int past = x.s.len - x.s.n;
+  x.pos_lo = past + static_cast<int>(g.group_div.div(x.row0));
+  x.pos_hi = x.rows ? past + static_cast<int>(g.group_div.div(x.row0 + x.rows - 1)) : -1;
+  return x;
+}
+__device__ __forceinline__ TileSpan span_of(const RowsArgs &g, const Group &x) {
+  TileSpan s{0, 0, 0};
+  if (x.rows == 0)
+    return s;
+  // A row group that sees nothing keeps one tile: its rows get zeros.
+  const int hi = max((x.pos_hi + kTile) / kTile, 1);
+  if (g.window > 0) {
+    const int lo = max(x.pos_lo + 1 - g.window, 0);
+    s.lo = lo / kTile;
+    s.sink = (min(g.sinks, lo) + kTile - 1) / kTile;
+    if (s.sink >= s.lo)
+      s.sink = s.lo = 0;
+  }
+  s.n = s.sink + hi - s.lo;
+  return s;
+}
+
+// A position in the sequence of all tiles: entry (sequence, row group), key
+// head, tile of that unit.
+struct Cursor {
+  int e, h, cnt, base, j;
+  __device__ __forceinline__ void start(const int *prefix, int entries, int kv_heads, int t) {
+    int lo = 0, hi = entries; // prefix[lo] <= t < prefix[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (prefix[mid] <= t)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    e = lo;
+    cnt = (prefix[e + 1] - prefix[e]) / kv_heads;
+    h = (t - prefix[e]) / cnt;
+    base = prefix[e] + h * cnt;
+    j = t - base;
+  }
+  __device__ __forceinline__ void next_unit(const int *prefix, int kv_heads) {
+    base += cnt;
+    j = 0;
+    if (++h == kv_heads) {
+      h = 0;
+      do
+        ++e;
+      while (prefix[e + 1] == prefix[e]);
+      cnt = (prefix[e + 1] - prefix[e]) / kv_heads;
+    }
+  }
+};
+
+template <int D, int NT> struct RowsLayout {
+  static constexpr int kStageBytes = kTile * (D + D / 4);
+  static constexpr int kStages = D == 128 && NT == 2 ? 3 : 4;
+  static constexpr int kCtasPerSm = D == 128 || NT == 2 ? 2 : 3;
+  static constexpr int kMaxGrid = kCtasPerSm * 148;
+  static constexpr int kRows = 8 * NT;
+  // Four warps' outputs, or the joining weights of every CTA's part.
+  static constexpr int kMergeFloats = kWarps * kRows * D > kMaxGrid * kRows ? kWarps * kRows * D : kMaxGrid * kRows;
+  static constexpr int kOffMerge = kStages * kStageBytes;
+  static constexpr int kOffStats = kOffMerge + kMergeFloats * 4; // m, l per warp and row
+  static constexpr int kOffBars = kOffStats + 2 * kWarps * kRows * 4;
+  static constexpr int kOffPrefix = kOffBars + 2 * kStages * 8 + 32;
+};
+template <int D, int NT> size_t rows_smem(int entries) {
+  return RowsLayout<D, NT>::kOffPrefix + (entries + 1 + kRowsThreads) * 4 + 1024;
+}
+
+// Key slot k (0..7) of a 16-key slice holds key order<D>(k), slot k + 8 key
+// order<D>(k) + 8: the order in which both products read the swizzled rows
+// without bank conflicts.
+template <int D> __device__ __forceinline__ int order(int k) {
+  return D == 128 ? ((k >> 1) & 1) + (k >> 2) * 4 + (k & 1) * 2 : (k >> 1) + (k & 1) * 4;
+}
+
+// Four channels of two keys (16-bit lanes a, b of x): values rounded to the
+// cache's type.
+template <bool BF16>
+__device__ __forceinline__ void restore4(uint32_t x, uint32_t scale, uint32_t low, uint32_t (&v)[4]) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162 *>(&scale);
+    const __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162 *>(&low);
+    const uint32_t off = 0x43004300u; // 128 + c
+    const __nv_bfloat162 o = *reinterpret_cast<const __nv_bfloat162 *>(&off);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c = ((x >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+      const __nv_bfloat162 r = __hfma2(__hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&c), o), s, m);
+      v[i] = *reinterpret_cast<const uint32_t *>(&r);
+    }
+  } else {
+    const __half2 s = *reinterpret_cast<const __half2 *>(&scale);
+    const __half2 m = *reinterpret_cast<const __half2 *>(&low);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t y = i < 2 ? x : x >> 8;
+      const uint32_t c = (y & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u; // 1024 + c or 1024 + 16 c
+      const __half2 w = *reinterpret_cast<const __half2 *>(&c);
+      const __half2 n = i & 1 ? __hfma2(w, __float2half2_rn(0.0625f), __float2half2_rn(-64.f))
+                              : __hsub2(w, __float2half2_rn(1024.f));
+      const __half2 r = __hfma2(n, s, m);
+      v[i] = *reinterpret_cast<const uint32_t *>(&r);
+    }
+  }
+}
+
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
+    rows_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ RowsArgs g) {
+  using L = RowsLayout<D, NT>;
+  constexpr int kRows = L::kRows, kStages = L::kStages;
+  constexpr int G = D / 32;    // groups per token
+  constexpr int kTiles = D / 16; // 16-channel tiles of the output
+  extern __shared__ uint8_t rows_smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(rows_smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  float *merge = reinterpret_cast<float *>(smem + L::kOffMerge);
+  float *stat_m = reinterpret_cast<float *>(smem + L::kOffStats);
+  float *stat_l = stat_m + kWarps * kRows;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::kOffBars);
+  uint64_t *empty = full + kStages;
+  volatile int *abort = reinterpret_cast<volatile int *>(empty + kStages);
+  volatile int *is_last = abort + 1;
+  int *prefix = reinterpret_cast<int *>(smem + L::kOffPrefix);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int entries = g.nb * g.nrg;
+  int *sums = prefix + entries + 1;
+  pdl_launch_dependents();
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, kWarps);
+    }
+    *abort = 0;
+    fence_barrier_init();
+  }
+  pdl_wait();
+
+  // Tiles before each entry.
+  {
+    const int per = (entries + kRowsThreads - 1) / kRowsThreads;
+    const int e0 = tid * per, e1 = min(e0 + per, entries);
+    int sum = 0;
+    for (int e = e0; e < e1; ++e) {
+      const int n = span_of(g, group_of<kRows>(g, g.b0 + e / g.nrg, g.rg0 + e % g.nrg)).n * g.kv_heads;
+      prefix[e + 1] = n;
+      sum += n;
+    }
+    sums[tid] = sum;
+    __syncthreads();
+    if (warp == 0) {
+      int v[kRowsThreads / 32], own = 0;
+#pragma unroll
+      for (int i = 0; i < kRowsThreads / 32; ++i) {
+        v[i] = own;
+        own += sums[lane * (kRowsThreads / 32) + i];
+      }
+      int run = own;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int x = __shfl_up_sync(~0u, run, o);
+        run += lane >= o ? x : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < kRowsThreads / 32; ++i)
+        sums[lane * (kRowsThreads / 32) + i] = run - own + v[i];
+    }
+    __syncthreads();
+    int run = sums[tid];
+    for (int e = e0; e < e1; ++e) {
+      run += prefix[e + 1];
+      prefix[e + 1] = run;
+    }
+    if (tid == 0)
+      prefix[0] = 0;
+    __syncthreads();
+  }
+  const int total = prefix[entries];
+  const int quota = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kMinTiles);
+  const int t0 = blockIdx.x * quota, t1 = min(t0 + quota, total);
+  if (t0 >= t1)
+    return;
+
+  Cursor cur;
+  cur.start(prefix, entries, g.kv_heads, t0);
+  if (warp == kWarps) {
+    // ------------------------------------------------------------ producer
+    const int page = 1 << g.t.page_shift;
+    int fill = 0;
+    for (int t = t0; t < t1;) {
+      const int b = g.b0 + cur.e / g.nrg;
+      const Group x = group_of<kRows>(g, b, g.rg0 + cur.e % g.nrg);
+      const TileSpan span = span_of(g, x);
+      const int end = min(t1, cur.base + cur.cnt);
+      bool ok = true;
+      for (; t < end; ++t, ++cur.j, ++fill) {
+        const int stage = fill % kStages;
+        const int pos = span.tile(cur.j) * kTile + lane * page;
+        const bool have = lane * page < kTile && pos < x.s.len;
+        const long long block =
+            have ? static_cast<long long>(kv4_page(g.t, b, pos)) * g.kv_heads + cur.h : 0;
+        if (fill >= kStages) {
+          ok = mbar_wait(empty + stage, (fill / kStages - 1) & 1, abort);
+          ok = __all_sync(~0u, ok);
+          if (!ok)
+            break;
+        }
+        const int pages = __popc(__ballot_sync(~0u, have));
+        if (lane == 0)
+          mbar_arrive_expect_tx(full + stage, pages * page * (D + D / 4));
+        __syncwarp();
+        if (have) {
+          uint8_t *dst = smem + stage * L::kStageBytes;
+          tma_load_4d(dst + lane * page * D, &codes_map, full + stage, 0, 0, 0, static_cast<int>(block));
+          bulk_load(dst + kTile * D + lane * page * (D / 4), g.pool + (block + 1) * page * (D + D / 4) - page * (D / 4),
+                    page * (D / 4), full + stage);
+        }
+      }
+      if (!ok) {
+        if (lane == 0)
+          *abort = 1;
+        break;
+      }
+      if (t < t1)
+        cur.next_unit(prefix, g.kv_heads);
+    }
+    if (lane == 0 && *abort) {
+      // No copy may land after the CTA is gone.
+      for (int f = max(fill - kStages, 0); f < fill; ++f) {
+        const long long c0 = clock64();
+        while (!mbar_try_wait(full + f % kStages, (f / kStages) & 1) && clock64() - c0 < kWaitBudgetCycles) {
+        }
+      }
+    }
+    return;
+  }
+
+  // -------------------------------------------------------------- consumers
+  const int lr = lane >> 2, lc = lane & 3; // row and column pair of a fragment
+  const int key_row = order<D>(lr);
+  const int key_a = order<D>(2 * lc), key_b = order<D>(2 * lc + 1);
+  // 16-byte chunk swizzle of a row of codes (see the tensor map).
+  auto swz = [](int key) { return D == 128 ? (key >> 1) & 3 : D == 64 ? (key >> 2) & 1 : 0; };
+  const int page_shift = g.t.page_shift, page = 1 << page_shift;
+  bool ok = true;
+  int fill = 0;
+  for (int t = t0; t < t1;) {
+    const int b = g.b0 + cur.e / g.nrg;
+    const Group x = group_of<kRows>(g, b, g.rg0 + cur.e % g.nrg);
+    const TileSpan span = span_of(g, x);
+
+    // Query rows: operand fragments, sums per group, factors of the scores.
+    uint32_t qf[NT][G][4];
+    float qsum[NT][G][2], factor[NT][2];
+    int pos[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = nt * 8 + lr;
+      uint4 w[G];
+      float most = 0.f;
+      {
+        const bool live = row < x.rows;
+        const uint32_t r = x.row0 + row;
+        const uint32_t i = g.group_div.div(r);
+        const uint16_t *p = g.q + (x.s.first + static_cast<long long>(i)) * g.q_stride +
+                            (cur.h * g.group + static_cast<int>(r - i * g.group)) * D + lc * 8;
+#pragma unroll
+        for (int c = 0; c < G; ++c)
+          w[c] = live ? *reinterpret_cast<const uint4 *>(p + c * 32) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int c = 0; c < G; ++c) {
+        const uint32_t in[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          most = fmaxf(most, fmaxf(fabsf(kv4_lo<BF16>(in[i])), fabsf(kv4_hi<BF16>(in[i]))));
+      }
+      most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
+      // up = 2^(13 - floor(log2 most)), within fp32's normal range.
+      const int ex = most > 0.f ? static_cast<int>(__float_as_uint(most) >> 23) : 127;
+      const float up = __uint_as_float(static_cast<uint32_t>(min(max(267 - ex, 1), 254)) << 23);
+      const float down = __fdiv_rn(16777216.f, up) * g.scale_log2; // 2^24 / up
+#pragma unroll
+      for (int c = 0; c < G; ++c) {
+        const uint32_t in[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+        float v[8], sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] = kv4_lo<BF16>(in[i]) * up;
+          v[2 * i + 1] = kv4_hi<BF16>(in[i]) * up;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          sum += v[i];
+        // Channels 0,4 | 1,5 of the first k step, 2,6 | 3,7 of the second:
+        // the pairs that one mask takes out of a word of codes. Odd ones
+        // meet 16 c.
+        qf[nt][c][0] = kv4_pack<false>(v[0], v[4]);
+        qf[nt][c][1] = kv4_pack<false>(v[1] * 0.0625f, v[5] * 0.0625f);
+        qf[nt][c][2] = kv4_pack<false>(v[2], v[6]);
+        qf[nt][c][3] = kv4_pack<false>(v[3] * 0.0625f, v[7] * 0.0625f);
+        sum += __shfl_xor_sync(~0u, sum, 1);
+        sum += __shfl_xor_sync(~0u, sum, 2);
+        sum *= 5.9604644775390625e-8f; // 2^-24, as the codes carry
+        qsum[nt][c][0] = __shfl_sync(~0u, sum, 8 * lc);
+        qsum[nt][c][1] = __shfl_sync(~0u, sum, 8 * lc + 4);
+      }
+      factor[nt][0] = __shfl_sync(~0u, down, 8 * lc);
+      factor[nt][1] = __shfl_sync(~0u, down, 8 * lc + 4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = nt * 8 + 2 * lc + i;
+        pos[nt][i] = r < x.rows ? x.s.len - x.s.n + static_cast<int>(g.group_div.div(x.row0 + r)) : -1;
+      }
+    }
+
+    float o[kTiles][NT][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        m[nt][i] = -INFINITY;
+        l[nt][i] = 0.f;
+      }
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[d][nt][i] = 0.f;
+    }
+
+    const int end = min(t1, cur.base + cur.cnt);
+    const bool from_start = t == cur.base, to_end = end == cur.base + cur.cnt;
+    for (; t < end; ++t, ++cur.j, ++fill) {
+      const int stage = fill % kStages;
+      if (!mbar_wait(full + stage, (fill / kStages) & 1, abort)) {
+        // Lost arrival: everybody stops waiting, the CTA runs out and the
+        // code is set.
+        ok = false;
+        *abort = 1;
+      }
+      const int key0 = span.tile(cur.j) * kTile + warp * 32;
+      const uint32_t st = sbase + stage * L::kStageBytes;
+      // Whether every row sees all of this warp's keys.
+      const bool clear = key0 + 31 <= x.pos_lo &&
+                         (g.window <= 0 || key0 > x.pos_hi - g.window || key0 + 32 <= g.sinks);
+      float s[2][NT][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int kk = warp * 32 + h * 16;
+        const int sub = kk >> page_shift, slot = kk & (page - 1);
+        const uint32_t codes = st + sub * page * D + slot * (D / 2);
+        const uint32_t params = st + kTile * D + sub * page * (D / 4) + slot * (D / 8);
+        const uint32_t row_a = codes + key_row * (D / 2), row_b = row_a + 8 * (D / 2);
+        uint32_t pa[G], pb[G];
+        {
+          const uint32_t at = params + key_row * (D / 8);
+          if constexpr (G == 4) {
+            const uint4 u = lds_v4(at), v = lds_v4(at + 8 * (D / 8));
+            pa[0] = u.x, pa[1] = u.y, pa[2] = u.z, pa[3] = u.w;
+            pb[0] = v.x, pb[1] = v.y, pb[2] = v.z, pb[3] = v.w;
+          } else if constexpr (G == 2) {
+            const uint2 u = lds_v2(at), v = lds_v2(at + 8 * (D / 8));
+            pa[0] = u.x, pa[1] = u.y;
+            pb[0] = v.x, pb[1] = v.y;
+          } else {
+            pa[0] = lds_u32(at);
+            pb[0] = lds_u32(at + 8 * (D / 8));
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[h][nt][i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < G; ++c) {
+          const uint32_t off = ((c ^ swz(key_row)) << 4) + 4 * lc;
+          const uint32_t wa = lds_u32(row_a + off), wb = lds_u32(row_b + off);
+          const uint32_t lo[4] = {wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u};
+          const uint32_t ya = wa >> 8, yb = wb >> 8;
+          const uint32_t hi[4] = {ya & 0x000F000Fu, yb & 0x000F000Fu, ya & 0x00F000F0u, yb & 0x00F000F0u};
+          const float sa = kv4_lo<BF16>(pa[c]), ma = kv4_hi<BF16>(pa[c]);
+          const float sb = kv4_lo<BF16>(pb[c]), mb = kv4_hi<BF16>(pb[c]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16(acc, lo, qf[nt][c][0], qf[nt][c][1]);
+            mma_f16(acc, hi, qf[nt][c][2], qf[nt][c][3]);
+            s[h][nt][0] += acc[0] * sa + qsum[nt][c][0] * ma;
+            s[h][nt][1] += acc[1] * sa + qsum[nt][c][1] * ma;
+            s[h][nt][2] += acc[2] * sb + qsum[nt][c][0] * mb;
+            s[h][nt][3] += acc[3] * sb + qsum[nt][c][1] * mb;
+          }
+        }
+      }
+      // Scores in powers of two; what a row does not see is replaced.
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[h][nt][i] *= factor[nt][i & 1];
+      if (!clear) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = key0 + h * 16 + key_row + (i >> 1) * 8;
+              const int p = pos[nt][i & 1];
+              const bool seen = key <= p && (g.window <= 0 || key > p - g.window || key < g.sinks);
+              s[h][nt][i] = seen ? s[h][nt][i] : -INFINITY;
+            }
+      }
+      bool raise = false;
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          top[nt][i] = fmaxf(fmaxf(s[0][nt][i], s[0][nt][i + 2]), fmaxf(s[1][nt][i], s[1][nt][i + 2]));
+          raise = raise || top[nt][i] > m[nt][i] + 8.f;
+        }
+      if (__any_sync(~0u, raise)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float v = fmaxf(top[nt][i], m[nt][i]);
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2)
+              v = fmaxf(v, __shfl_xor_sync(~0u, v, d));
+            const float r = v > m[nt][i] ? ex2_ftz(m[nt][i] - v) : 1.f;
+            m[nt][i] = v;
+            l[nt][i] *= r;
+#pragma unroll
+            for (int d = 0; d < kTiles; ++d) {
+              o[d][nt][i] *= r;
+              o[d][nt][i + 2] *= r;
+            }
+          }
+      }
+      uint32_t pf[2][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        // Nothing seen yet: every score is -inf, and so must its power be 0.
+        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float p0 = ex2_ftz(s[h][nt][0] - m0), p1 = ex2_ftz(s[h][nt][1] - m1);
+          const float p2 = ex2_ftz(s[h][nt][2] - m0), p3 = ex2_ftz(s[h][nt][3] - m1);
+          l[nt][0] += p0 + p2;
+          l[nt][1] += p1 + p3;
+          pf[h][nt][0] = transpose8x8(kv4_pack<BF16>(p0, p1));
+          pf[h][nt][1] = transpose8x8(kv4_pack<BF16>(p2, p3));
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int kk = warp * 32 + h * 16;
+        const int sub = kk >> page_shift, slot = kk & (page - 1);
+        const uint32_t codes = st + sub * page * D + page * (D / 2) + slot * (D / 2);
+        const uint32_t params = st + kTile * D + sub * page * (D / 4) + page * (D / 8) + slot * (D / 8) +
+                                (D == 128 ? lr >> 1 : D == 64 ? lr >> 2 : 0) * 4;
+        // Channel rows lr and lr + 8 of every tile; the keys of both pairs.
+        uint32_t scale[2], low[2], w[2][2][D == 128 ? 2 : 1];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int ka = key_a + 8 * u, kb = key_b + 8 * u;
+          uint32_t pa = lds_u32(params + ka * (D / 8)), pb = lds_u32(params + kb * (D / 8));
+          if (!clear) {
+            const int key = key0 + h * 16;
+            pa = key + ka < x.s.len ? pa : 0u;
+            pb = key + kb < x.s.len ? pb : 0u;
+          }
+          scale[u] = __byte_perm(pa, pb, 0x5410);
+          low[u] = __byte_perm(pa, pb, 0x7632);
+          const uint32_t ra = codes + ka * (D / 2), rb = codes + kb * (D / 2);
+          if constexpr (D == 128) {
+            const uint2 a = lds_v2(ra + (((lr >> 1) ^ swz(key_a)) << 4) + (lr & 1) * 8);
+            const uint2 c = lds_v2(rb + (((lr >> 1) ^ swz(key_b)) << 4) + (lr & 1) * 8);
+            w[u][0][0] = a.x, w[u][0][1] = a.y;
+            w[u][1][0] = c.x, w[u][1][1] = c.y;
+          } else if constexpr (D == 64) {
+            w[u][0][0] = lds_u32(ra + (((lr >> 2) ^ swz(key_a)) << 4) + (lr & 3) * 4);
+            w[u][1][0] = lds_u32(rb + (((lr >> 2) ^ swz(key_b)) << 4) + (lr & 3) * 4);
+          } else {
+            w[u][0][0] = lds_u16(ra + lr * 2);
+            w[u][1][0] = lds_u16(rb + lr * 2);
+          }
+        }
+        if constexpr (D == 32) {
+          // Channels 4 lr .. 4 lr + 3: tile t takes t and t + 2.
+          uint32_t v0[4], v1[4];
+          restore4<BF16>(__byte_perm(w[0][0][0], w[0][1][0], 0x5410), scale[0], low[0], v0);
+          restore4<BF16>(__byte_perm(w[1][0][0], w[1][1][0], 0x5410), scale[1], low[1], v1);
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            const uint32_t a[4] = {v0[d], v0[d + 2], v1[d], v1[d + 2]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if constexpr (BF16)
+                mma_bf16(o[d][nt], a, pf[h][nt][0], pf[h][nt][1]);
+              else
+                mma_f16(o[d][nt], a, pf[h][nt][0], pf[h][nt][1]);
+            }
+          }
+        } else {
+          // Word i holds channels 8 i .. 8 i + 7 of this thread's run; tile
+          // 4 i + t takes channels t and t + 4 of it.
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            uint32_t v0[4], v1[4], v2[4], v3[4];
+            restore4<BF16>(__byte_perm(w[0][0][i], w[0][1][i], 0x5410), scale[0], low[0], v0);
+            restore4<BF16>(__byte_perm(w[0][0][i], w[0][1][i], 0x7632), scale[0], low[0], v1);
+            restore4<BF16>(__byte_perm(w[1][0][i], w[1][1][i], 0x5410), scale[1], low[1], v2);
+            restore4<BF16>(__byte_perm(w[1][0][i], w[1][1][i], 0x7632), scale[1], low[1], v3);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              const uint32_t a[4] = {v0[d], v1[d], v2[d], v3[d]};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if constexpr (BF16)
+                  mma_bf16(o[4 * i + d][nt], a, pf[h][nt][0], pf[h][nt][1]);
+                else
+                  mma_f16(o[4 * i + d][nt], a, pf[h][nt][0], pf[h][nt][1]);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(empty + stage);
+    }
+
+    // ---- the four warps' parts of this unit into one
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2)
+          l[nt][i] += __shfl_xor_sync(~0u, l[nt][i], d);
+        if (lr == 0) {
+          stat_m[warp * kRows + nt * 8 + 2 * lc + i] = m[nt][i];
+          stat_l[warp * kRows + nt * 8 + 2 * lc + i] = l[nt][i];
+        }
+      }
+    consumer_barrier();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = nt * 8 + 2 * lc + i;
+        float top = stat_m[row];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w)
+          top = fmaxf(top, stat_m[w * kRows + row]);
+        const float r = m[nt][i] == -INFINITY ? 0.f : ex2_ftz(m[nt][i] - top);
+        // This thread's channels of the row are D / 8 neighbours.
+        float *dst = merge + (warp * kRows + row) * D + lr * (D / 8);
+        float v[D / 8];
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) {
+          const int at = D == 32 ? d : (d / 4) * 8 + d % 4;
+          v[at] = o[d][nt][i] * r;
+          v[at + (D == 32 ? 2 : 4)] = o[d][nt][i + 2] * r;
+        }
+#pragma unroll
+        for (int c = 0; c < D / 8; c += 4)
+          *reinterpret_cast<float4 *>(dst + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+      }
+    consumer_barrier();
+    const bool whole = from_start && to_end;
+    // A CTA leaves at most two parts: of the unit it came in on and of the
+    // one it goes out on.
+    float *part = g.parts + static_cast<long long>(blockIdx.x * 2 + (from_start ? 1 : 0)) * kPartFloats;
+    auto store = [&](int row, int d, float4 v) {
+      if (row >= x.rows)
+        return;
+      const uint32_t r = x.row0 + row;
+      const uint32_t i = g.group_div.div(r);
+      const long long at = ((x.s.first + static_cast<long long>(i)) * g.heads + cur.h * g.group +
+                            static_cast<int>(r - i * g.group)) * D + d;
+      *reinterpret_cast<uint2 *>(g.out + at) = make_uint2(kv4_pack<BF16>(v.x, v.y), kv4_pack<BF16>(v.z, v.w));
+    };
+#pragma unroll
+    for (int it = tid; it < kRows * D / 4; it += 32 * kWarps) {
+      const int row = it / (D / 4), d = it % (D / 4) * 4;
+      float4 v = *reinterpret_cast<const float4 *>(merge + row * D + d);
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) {
+        const float4 y = *reinterpret_cast<const float4 *>(merge + (w * kRows + row) * D + d);
+        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+      }
+      float top = stat_m[row];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w)
+        top = fmaxf(top, stat_m[w * kRows + row]);
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        sum += top == -INFINITY ? 0.f : stat_l[w * kRows + row] * ex2_ftz(stat_m[w * kRows + row] - top);
+      if (whole) {
+        const float r = sum > 0.f ? __fdividef(1.f, sum) : sum; // NaN stays NaN
+        store(row, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
+      } else {
+        *reinterpret_cast<float4 *>(part + row * D + d) = v;
+        if (d == 0) {
+          part[kRows * D + row] = top;
+          part[kRows * D + kRows + row] = sum;
+        }
+      }
+    }
+    if (!whole) {
+      // ---- the last CTA to finish joins the unit's parts
+      const int first = cur.base / quota, parts = (cur.base + cur.cnt - 1) / quota - first + 1;
+      __threadfence();
+      consumer_barrier();
+      if (tid == 0) {
+        int *c = g.counters + cur.e * g.kv_heads + cur.h;
+        const int seen = atomicAdd(c, 1);
+        *is_last = seen == parts - 1;
+        if (seen == parts - 1)
+          *c = 0;
+      }
+      consumer_barrier();
+      if (*is_last) {
+        __threadfence();
+        auto part_of = [&](int i) {
+          // The unit's first CTA went out on it unless the unit starts there.
+          const int cta = first + i;
+          const bool began = cur.base >= cta * quota;
+          return g.parts + static_cast<long long>(cta * 2 + (began ? 1 : 0)) * kPartFloats;
+        };
+        for (int i = tid; i < parts * kRows; i += 32 * kWarps)
+          merge[i] = __ldcg(part_of(i / kRows) + kRows * D + i % kRows);
+        consumer_barrier();
+        for (int it = tid; it < kRows * D / 4; it += 32 * kWarps) {
+          const int row = it / (D / 4), d = it % (D / 4) * 4;
+          float top = -INFINITY;
+          for (int i = 0; i < parts; ++i)
+            top = fmaxf(top, merge[i * kRows + row]);
+          float sum = 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int i = 0; i < parts; ++i) {
+            const float *p = part_of(i);
+            const float4 y = __ldcg(reinterpret_cast<const float4 *>(p + row * D + d));
+            const float ly = __ldcg(p + kRows * D + kRows + row);
+            const float my = merge[i * kRows + row];
+            const float r = my == -INFINITY ? 0.f : ex2_ftz(my - top);
+            sum += ly * r;
+            v.x += y.x * r, v.y += y.y * r, v.z += y.z * r, v.w += y.w * r;
+          }
+          const float r = sum > 0.f ? __fdividef(1.f, sum) : sum;
+          store(row, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
+        }
+      }
+    }
+    consumer_barrier();
+    if (t < t1)
+      cur.next_unit(prefix, g.kv_heads);
+  }
+  if (!ok && lane == 0)
+    kv4_fault(g.t, kErrRowsWait);
+}
+
+template <int D, int NT, bool BF16>
+cudaError_t launch_rows(const CUtensorMap &map, const RowsArgs &g, cudaStream_t stream) {
+  auto *kernel = rows_kernel<D, NT, BF16>;
+  const size_t smem = rows_smem<D, NT>(g.nb * g.nrg);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess)
+    return e;
+  const int grid = std::min(RowsLayout<D, NT>::kCtasPerSm * sm_count(), RowsLayout<D, NT>::kMaxGrid);
+  return launch_pdl(kernel, grid, kRowsThreads, smem, stream, map, g);
+}
+
+} // namespace
+
+size_t kv4_workspace_bytes() {
+  return static_cast<size_t>(kMaxUnits) * 4 + static_cast<size_t>(kMaxCtas) * 2 * kPartFloats * 4;
+}
+
+cudaError_t kv4_attend_rows(const Kv4Cache &c, const Kv4Tokens &t, const Kv4Attention &a, cudaStream_t stream) {
+  RowsArgs g{};
+  g.t = t;
+  g.pool = c.pool;
+  g.q = static_cast<const uint16_t *>(a.q);
+  g.out = static_cast<uint16_t *>(a.out);
+  g.q_stride = a.q_stride;
+  g.heads = a.heads;
+  g.kv_heads = c.kv_heads;
+  g.group = a.heads / c.kv_heads;
+  g.group_div = FastDiv(g.group);
+  g.window = a.window;
+  g.sinks = a.sinks;
+  g.scale_log2 = a.scale * kLog2e;
+  g.counters = static_cast<int *>(a.workspace);
+  g.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(a.workspace) + static_cast<size_t>(kMaxUnits) * 4);
+  const int D = c.head_dim, P = c.page_size;
+  const cuuint64_t half = D / 2, block = kv4_block_bytes(P, D);
+  const cuuint64_t dims[4] = {half, static_cast<cuuint64_t>(P), 2, static_cast<cuuint64_t>(c.pages) * c.kv_heads};
+  const cuuint64_t strides[3] = {half, half * P, block};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(half), static_cast<cuuint32_t>(P), 2, 1};
+  CUtensorMap map;
+  if (!encode_u8_map(&map, c.pool, 4, dims, strides, box, D == 128 ? 64 : D == 64 ? 32 : 0))
+    return cudaErrorInvalidValue;
+  // Eight query rows a unit where no sequence has more, else sixteen (the
+  // cache is then read once per sixteen rows).
+  const long long rows = static_cast<long long>(t.max_new) * g.group;
+  const int nt = rows <= 8 ? 1 : 2;
+  const long long groups = (rows + 8 * nt - 1) / (8 * nt);
+  const long long most = std::min<long long>(kMaxEntries, kMaxUnits / c.kv_heads);
+  const int per_rg = static_cast<int>(std::min<long long>(groups, most));
+  const int per_b = static_cast<int>(std::max<long long>(1, most / per_rg));
+  for (int b = 0; b < t.batch; b += per_b)
+    for (long long rg = 0; rg < groups; rg += per_rg) {
+      g.b0 = b;
+      g.nb = std::min(per_b, t.batch - b);
+      g.rg0 = static_cast<int>(rg);
+      g.nrg = static_cast<int>(std::min<long long>(per_rg, groups - rg));
+      cudaError_t e;
+      switch (D * 4 + (nt - 1) * 2 + c.bf16) {
+      case 128: e = launch_rows<32, 1, false>(map, g, stream); break;
+      case 129: e = launch_rows<32, 1, true>(map, g, stream); break;
+      case 130: e = launch_rows<32, 2, false>(map, g, stream); break;
+      case 131: e = launch_rows<32, 2, true>(map, g, stream); break;
+      case 256: e = launch_rows<64, 1, false>(map, g, stream); break;
+      case 257: e = launch_rows<64, 1, true>(map, g, stream); break;
+      case 258: e = launch_rows<64, 2, false>(map, g, stream); break;
+      case 259: e = launch_rows<64, 2, true>(map, g, stream); break;
+      case 512: e = launch_rows<128, 1, false>(map, g, stream); break;
+      case 513: e = launch_rows<128, 1, true>(map, g, stream); break;
+      case 514: e = launch_rows<128, 2, false>(map, g, stream); break;
+      case 515: e = launch_rows<128, 2, true>(map, g, stream); break;
+      default: e = cudaErrorInvalidValue;
+      }
+      if (e != cudaSuccess)
+        return e;
+    }
+  return cudaSuccess;
+}
+
+} // namespace pb2

@@ -418,6 +418,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 bool encode_fp16_map(CUtensorMap *m, const void *base, int rank,
                      const cuuint64_t *dims, const cuuint64_t *strides,
                      const cuuint32_t *box, bool swizzle128);
+// The same for bytes, with a swizzle span of 64, 32 or 0 (none) bytes.
+bool encode_u8_map(CUtensorMap *m, const void *base, int rank,
+                   const cuuint64_t *dims, const cuuint64_t *strides,
+                   const cuuint32_t *box, int swizzle_bytes);
 
 // Unsigned division by a run-time invariant for dividends below 2^31
 // (Granlund & Montgomery, "Division by invariant integers using

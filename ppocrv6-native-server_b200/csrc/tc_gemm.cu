@@ -1021,6 +1021,20 @@ bool encode_fp16_map(CUtensorMap *m, const void *base, int rank,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_u8_map(CUtensorMap *m, const void *base, int rank, const cuuint64_t *dims, const cuuint64_t *strides,
+                   const cuuint32_t *box, int swizzle_bytes) {
+  EncodeTiled fn = encoder();
+  if (!fn)
+    return false;
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void *>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE,
+            swizzle_bytes == 64   ? CU_TENSOR_MAP_SWIZZLE_64B
+            : swizzle_bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
+                                  : CU_TENSOR_MAP_SWIZZLE_NONE,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 cudaError_t tc_gemm(const half *A, int M, int K, int lda, const half *W, int N,
                     int ldw, const GemmEpilogue &epi, cudaStream_t stream) {
   if (M <= 0 || N <= 0)

@@ -26,7 +26,8 @@ def lib_path() -> Path:
 
 
 # (name, restype, argtypes) for every function in include/ppocr_b200_head.h,
-# include/ppocr_b200_ops.h and include/ppocr_b200_preprocess.h.
+# include/ppocr_b200_ops.h, include/ppocr_b200_preprocess.h and
+# include/ppocr_b200_decode.h.
 V, I, F, S, L = c_void_p, c_int, c_float, c_size_t, c_longlong
 PI, PF = POINTER(c_int), POINTER(c_float)
 SIGNATURES = {
@@ -76,6 +77,13 @@ SIGNATURES = {
     "ppocr_b200_batch_roi_warp": (I, [V, S, I, I, V, V, V, I, I, I, I, V]),
     "ppocr_b200_roi_warp": (I, [V, S, I, I, V, V, V, I, I, I, I, I, V]),
     "ppocr_b200_line_tensors": (I, [V, V, V, V, V, I, I, V, I, V]),
+    # include/ppocr_b200_decode.h
+    "ppocr_b200_kv4_block_bytes": (S, [I, I]),
+    "ppocr_b200_kv4_append": (I, [V, V, L, V, L, V, I, V, V, I, I, I, V]),
+    "ppocr_b200_kv4_read": (I, [V, V, V, V, I, V, V, I, I, I, V]),
+    "ppocr_b200_kv4_workspace_bytes": (S, []),
+    "ppocr_b200_kv4_attention": (I, [V, V, L, V, I, F, I, I, V, I, V, V, I, I, I, V, V]),
+    "ppocr_b200_sample": (I, [V, I, L, I, I, V, V, V, V, V, V, V, V, V]),
 }
 PREP_F32_NCHW, PREP_F16_NHWC = 0, 1
 
@@ -133,6 +141,19 @@ class PpocrModelInfo(ctypes.Structure):
         ("output_element_bytes", c_int),
         ("weight_file_bytes", c_size_t),
         ("scratch_bytes", c_size_t),
+    ]
+
+
+class PpocrKv4Cache(ctypes.Structure):
+    """Layout of PpocrKv4Cache (include/ppocr_b200_decode.h)."""
+
+    _fields_ = [
+        ("pool", c_void_p),
+        ("pages", c_longlong),
+        ("page_size", c_int),
+        ("kv_heads", c_int),
+        ("head_dim", c_int),
+        ("type", c_int),
     ]
 
 
