@@ -1,22 +1,41 @@
-// Token sampling: temperature, top-k, top-p, min-p and the draw, one CTA per
-// row of logits.
+// Token sampling: temperature, top-k, top-p, min-p and the draw.
 //
 // Masses are whole numbers, floor(exp(-(max - x) / T) * 2^32): every sum is
 // exact whatever its order, so the result depends on no split of the work.
 // What stays of a row is always a prefix of its order (larger logits first,
 // equal ones by index), so it is described by one logit value (as an
 // order-preserving 32-bit key), and by how many of the logits equal to it
-// stay. That value is found digit by digit from the top: a histogram of
-// counts and masses over 256 values of one byte of the key, among the logits
-// that agree with the digits found so far.
+// stay; min-p is a bound on the mass of its own.
+//
+// One row is one cluster of 1 to 8 CTAs and is read once: every CTA keeps its
+// run of the row in shared memory, each warp a run of that, and the CTAs
+// exchange sums through distributed shared memory.
+//  1. the maximum, the masses and their sum;
+//  2. a bound below which the prefix cannot end: for top-k the smallest
+//     logit L such that every warp has its share of k logits at or above it;
+//     for top-p the mass (1 - p) sum / V (all that is lighter cannot make up
+//     1 - p together), or min-p where that is more;
+//  3. a histogram of counts and masses of what passes the bound, over 512
+//     steps of max - x: its running sums say in which step the prefix ends;
+//  4. the logits of that step, sorted and summed in order (every CTA does
+//     this for itself); a step with more than fit, as of many equal logits,
+//     is resolved digit by digit of the key instead, over the row in memory;
+//  5. the draw: a scan of the threads' kept masses, in index order.
+// Rows longer than a cluster's shared memory take the digit search alone.
+// Bound by the instructions of step 1 (a division, an exponential and a 64-bit
+// sum per logit); the steps after it touch only what passes a comparison,
+// each lane working off its own hits (a mask of 32 logits a lane) so that few
+// hits cost few turns of the warp.
 #include "kernels.h"
 #include "ptx.cuh"
+#include <algorithm>
+#include <climits>
 #include <cuda_bf16.h>
 
 namespace pb2 {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024; // of the digit search over long rows
 using u64 = unsigned long long;
 
 template <int TYPE> __device__ __forceinline__ float logit(const void *row, int i) {
@@ -27,11 +46,11 @@ template <int TYPE> __device__ __forceinline__ float logit(const void *row, int 
     x = __bfloat162float(static_cast<const __nv_bfloat16 *>(row)[i]);
   else
     x = __half2float(static_cast<const half *>(row)[i]);
-  return x == x ? x + 0.f : -INFINITY; // NaN never wins; -0 equals 0
+  return x == x ? x : -INFINITY; // NaN never wins
 }
 // Larger logits, larger keys.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f); // -0 equals 0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
@@ -54,12 +73,13 @@ struct Prefix {
   u64 mass;
 };
 
-struct Shared {
+struct Digits {
   unsigned count[256];
   u64 mass[256];
+};
+struct Shared : Digits {
   u64 warp[32];
   int warp_n[32];
-  Prefix found;
 };
 
 template <typename T> __device__ __forceinline__ T block_sum(T v, T *slots) {
@@ -81,18 +101,18 @@ template <typename T> __device__ __forceinline__ T block_sum(T v, T *slots) {
 // The first `want` logits of the row's order (by_mass false), or the fewest
 // whose mass reaches `want` > 0 (by_mass true).
 template <int TYPE>
-__device__ Prefix select(const void *row, int vocab, float top, float t, bool by_mass, u64 want, Shared &sh) {
+__device__ __noinline__ Prefix select(const void *row, int vocab, float top, float t, bool by_mass, u64 want, Digits &sh) {
   uint32_t prefix = 0;
   u64 before = 0; // mass of the logits above the digits found so far
   int above = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
     __syncthreads();
-    for (int i = threadIdx.x; i < 256; i += kThreads) {
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) {
       sh.count[i] = 0;
       sh.mass[i] = 0;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < vocab; i += kThreads) {
+    for (int i = threadIdx.x; i < vocab; i += blockDim.x) {
       const float x = logit<TYPE>(row, i);
       const uint32_t k = key_of(x);
       if (shift == 24 || (k >> (shift + 8)) == prefix) {
@@ -128,7 +148,7 @@ __device__ Prefix select(const void *row, int vocab, float top, float t, bool by
   return p;
 }
 
-template <int TYPE> __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
+template <int TYPE> __global__ void __launch_bounds__(kThreads) sample_long_kernel(const __grid_constant__ SampleArgs a) {
   __shared__ Shared sh;
   pdl_begin();
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -249,13 +269,672 @@ template <int TYPE> __global__ void __launch_bounds__(kThreads) sample_kernel(co
   }
 }
 
+// ------------------------------------------------- one cluster, one row
+constexpr int kBins = 512;
+constexpr int kCap = 1024;    // logits that are sorted at most
+constexpr int kMostCtas = 8;
+constexpr float kReach = 22.2f; // exp(-22.2) < 2^-32: no mass past it
+
+struct Part { // one CTA's sums
+  u64 all, likely; // mass; mass at or above min-p
+  int likely_n;
+  uint32_t bound;  // smallest key that passes the top-k bound
+};
+struct Ends {
+  float top, low; // largest and smallest finite logit
+};
+struct ClusterShared {
+  union {
+    struct {
+      unsigned count[kBins], lo[kBins], hi[kBins];
+    } bins;
+    Digits digits;
+  };
+  u64 keys[2][kCap]; // of the step where top-k and top-p end
+  int taken[2];
+  Ends ends[kMostCtas], warp_ends[32];
+  Part part[kMostCtas], warp_part[32];
+  u64 drawn[kMostCtas];
+  int tied[kMostCtas];
+  u64 warp[32];
+  int warp_n[32];
+  u64 edge_mass;
+  int edge_bin, edge_count, edge_before;
+  Prefix found;
+};
+
+// This cluster's CTAs.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same shared variable in CTA `rank`, as a generic pointer.
+template <typename T> __device__ __forceinline__ T *remote(T *p, uint32_t rank) {
+  uint64_t q;
+  asm volatile("mapa.u64 %0, %1, %2;" : "=l"(q) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
+  return reinterpret_cast<T *>(q);
+}
+
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+#pragma unroll
+  for (int o = 16; o; o /= 2)
+    v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+template <typename T> __device__ __forceinline__ T warp_scan(T v) { // inclusive
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const T y = __shfl_up_sync(~0u, v, o);
+    v += lane >= o ? y : 0;
+  }
+  return v;
+}
+// Exclusive sums over the block, in place; returns the block's.
+__device__ __forceinline__ void block_scan(u64 &m, int &n, ClusterShared &sh, u64 &m_total, int &n_total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const u64 mi = warp_scan(m);
+  const int ni = warp_scan(n);
+  __syncthreads();
+  if (lane == 31) {
+    sh.warp[warp] = mi;
+    sh.warp_n[warp] = ni;
+  }
+  __syncthreads();
+  const u64 mw = warp_scan(lane < warps ? sh.warp[lane] : 0);
+  const int nw = warp_scan(lane < warps ? sh.warp_n[lane] : 0);
+  m_total = __shfl_sync(~0u, mw, 31);
+  n_total = __shfl_sync(~0u, nw, 31);
+  const u64 mb = __shfl_sync(~0u, mw, max(warp - 1, 0));
+  const int nb = __shfl_sync(~0u, nw, max(warp - 1, 0));
+  m = mi - m + (warp ? mb : 0);
+  n = ni - n + (warp ? nb : 0);
+}
+
+// Sorts `n` collected keys (logit key, then lower index first), of which
+// `count` logits of mass `mass` lie before, and ends the prefix after `want`
+// logits (by_mass false) or where its mass reaches `want`. Run by a whole CTA.
+__device__ __noinline__ Prefix resolve(ClusterShared &sh, u64 *keys, int n, int count, u64 mass, bool by_mass, u64 want,
+                                       float top, float t) {
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
+  auto mass_at = [&](u64 key) { return mass_of(share_of(value_of(static_cast<uint32_t>(key >> 32)), top, t)); };
+  if (n <= 32) {
+    if (tid < 32) {
+      u64 key = lane < n ? keys[lane] : 0;
+#pragma unroll
+      for (int run = 2; run <= 32; run *= 2)
+#pragma unroll
+        for (int gap = run / 2; gap; gap /= 2) {
+          const u64 y = __shfl_xor_sync(~0u, key, gap);
+          const bool larger = ((lane & gap) == 0) == ((lane & run) == 0); // this lane keeps the larger
+          key = (key > y) == larger ? key : y;
+        }
+      const u64 own = lane < n ? mass_at(key) : 0;
+      const u64 cum = mass + warp_scan(own);
+      const unsigned ends = __ballot_sync(
+          ~0u, lane < n && (by_mass ? cum >= want : static_cast<u64>(count + lane + 1) >= want));
+      const int at = ends ? __ffs(ends) - 1 : n - 1;
+      const uint32_t edge = static_cast<uint32_t>(__shfl_sync(~0u, key, at) >> 32);
+      const unsigned same = __ballot_sync(~0u, lane < n && static_cast<uint32_t>(key >> 32) == edge);
+      if (lane == at)
+        sh.found = Prefix{edge, at - (__ffs(same) - 1) + 1, count + at + 1, cum};
+    }
+    __syncthreads();
+    return sh.found;
+  }
+  int size = 64;
+  while (size < n)
+    size *= 2;
+  for (int i = n + tid; i < size; i += threads)
+    keys[i] = 0;
+  __syncthreads();
+  for (int run = 2; run <= size; run *= 2)
+    for (int gap = run / 2; gap; gap /= 2) {
+      for (int i = tid; i < size / 2; i += threads) {
+        const int a = 2 * i - (i & (gap - 1)), b = a + gap;
+        const u64 x = keys[a], y = keys[b];
+        if ((x < y) == ((a & run) == 0)) {
+          keys[a] = y;
+          keys[b] = x;
+        }
+      }
+      __syncthreads();
+    }
+  const int per = (n + threads - 1) / threads;
+  const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+  u64 before = 0, total;
+  int unused = 0, unused_total;
+  for (int i = i0; i < i1; ++i)
+    before += mass_at(keys[i]);
+  block_scan(before, unused, sh, total, unused_total);
+  u64 cum = mass + before;
+  for (int i = i0; i < i1; ++i) {
+    const u64 m = mass_at(keys[i]);
+    const bool ends = by_mass ? cum < want && (cum + m >= want || i == n - 1)
+                              : static_cast<u64>(count + i + 1) == want;
+    cum += m;
+    if (ends) {
+      const uint32_t key = static_cast<uint32_t>(keys[i] >> 32);
+      int a = 0, b = i; // first place of this key
+      while (a < b) {
+        const int mid = (a + b) / 2;
+        if (static_cast<uint32_t>(keys[mid] >> 32) > key)
+          a = mid + 1;
+        else
+          b = mid;
+      }
+      sh.found = Prefix{key, i - a + 1, count + i + 1, cum};
+    }
+  }
+  __syncthreads();
+  return sh.found;
+}
+
+constexpr int kRowThreads = 512;
+
+template <int TYPE>
+__global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid_constant__ SampleArgs a) {
+  extern __shared__ uint4 granules[]; // this CTA's run of the row
+  __shared__ ClusterShared sh;
+  constexpr int kSize = TYPE == LOGIT_F32 ? 4 : 2;
+  constexpr int kVec = 16 / kSize;      // logits a granule of 16 bytes
+  constexpr int kGroup = 32 / kVec;     // granules a lane masks at once
+  constexpr int kWarps = kRowThreads / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ctas = gridDim.x, rank = cluster_rank();
+  const int r = blockIdx.y, V = a.vocab;
+  pdl_launch_dependents();
+  for (int i = tid; i < kBins; i += kRowThreads)
+    sh.bins.count[i] = sh.bins.lo[i] = sh.bins.hi[i] = 0;
+  if (tid < 2)
+    sh.taken[tid] = 0;
+  pdl_wait();
+  const char *row = static_cast<const char *>(a.logits) + static_cast<long long>(r) * a.stride * kSize;
+  // The row in granules: the first and the last may hold neighbours' logits,
+  // which become -inf (no mass, and last among equals by their index).
+  const int head = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) / kSize;
+  const uint4 *base = reinterpret_cast<const uint4 *>(row - head * kSize);
+  const int all_g = (V + head + kVec - 1) / kVec;
+  const int cta_g = (all_g + ctas - 1) / ctas;
+  const int warp_g = (cta_g + kWarps - 1) / kWarps;
+  const int cta0 = rank * cta_g, cta1 = min(cta0 + cta_g, all_g);
+  // This warp's granules, within the CTA's.
+  const int g0 = min(warp * warp_g, max(cta1 - cta0, 0)), g1 = max(min(g0 + warp_g, cta1 - cta0), g0);
+  auto index_of = [&](int g, int j) { return (cta0 + g) * kVec + j - head; };
+  auto at = [&](const uint4 &w, int j) {
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (TYPE == LOGIT_F32)
+      return __uint_as_float(in[j]);
+    else if constexpr (TYPE == LOGIT_BF16)
+      return __uint_as_float(j & 1 ? in[j / 2] & 0xFFFF0000u : in[j / 2] << 16);
+    else
+      return __half2float(__ushort_as_half(static_cast<unsigned short>(j & 1 ? in[j / 2] >> 16 : in[j / 2] & 0xFFFFu)));
+  };
+  auto one = [&](int g, int j) { // one logit from shared memory
+    if constexpr (TYPE == LOGIT_F32)
+      return reinterpret_cast<const float *>(granules + g)[j];
+    const uint32_t u = reinterpret_cast<const uint16_t *>(granules + g)[j];
+    if constexpr (TYPE == LOGIT_BF16)
+      return __uint_as_float(u << 16);
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(u)));
+  };
+
+  float t = a.temperature ? a.temperature[r] : 1.f;
+  int k = a.top_k ? a.top_k[r] : 0;
+  const float tp = a.top_p ? a.top_p[r] : 1.f;
+  float mp = a.min_p ? a.min_p[r] : 0.f;
+  k = k <= 0 || k > V ? V : k;
+  if (!(t > 0.f)) {
+    t = 1.f;
+    k = 1;
+  }
+  if (mp > 1.f) { // only the first passes
+    k = 1;
+    mp = 1.f;
+  }
+  mp = mp > 0.f ? mp : 0.f;
+  const u64 p24 = __float2ull_rz(fminf(fmaxf(tp, 0.f), 1.f) * 16777216.f);
+  const u64 u24 = min(__float2ull_rz(fminf(fmaxf(a.uniform[r], 0.f), 1.f) * 16777216.f), 16777215ull);
+  const bool by_k = k < V && k > 1, by_p = k > 1 && p24 < (1ull << 24);
+
+  // ---- 1. maximum
+  float top = -INFINITY, low = INFINITY;
+  {
+    constexpr uint32_t kNegInf = TYPE == LOGIT_F32 ? 0xFF800000u : TYPE == LOGIT_BF16 ? 0xFF80u : 0xFC00u;
+#pragma unroll 4
+    for (int g = g0 + lane; g < g1; g += 32) {
+      uint4 w = __ldg(base + cta0 + g);
+      uint32_t in[4] = {w.x, w.y, w.z, w.w};
+      const bool edge = index_of(g, 0) < 0 || index_of(g, kVec) > V;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const float v = at(w, j);
+        bool bad = !(v == v);
+        if (edge)
+          bad = bad || index_of(g, j) < 0 || index_of(g, j) >= V;
+        if (bad) {
+          if constexpr (TYPE == LOGIT_F32)
+            in[j] = kNegInf;
+          else
+            in[j / 2] = j & 1 ? (in[j / 2] & 0xFFFFu) | kNegInf << 16 : (in[j / 2] & 0xFFFF0000u) | kNegInf;
+        } else {
+          top = fmaxf(top, v);
+          low = v > -INFINITY ? fminf(low, v) : low;
+        }
+      }
+      granules[g] = make_uint4(in[0], in[1], in[2], in[3]);
+    }
+  }
+  __syncwarp();
+  // Every warp whose run lies wholly inside the row has j logits at or above
+  // the j-th largest of its lanes' maxima.
+  uint32_t bound = 0xFFFFFFFFu;
+  {
+    // Runs of warp_g granules of a CTA's cta_g: whole ones per full CTA.
+    const int whole = cta_g / warp_g;
+    const int full = max((all_g / cta_g) * whole - 2, 0);
+    const int share = full > 0 ? (k + full - 1) / full : 33;
+    if (by_k && share <= 16 && warp_g >= 32) {
+      const bool inside = g1 - g0 == warp_g && index_of(g0, 0) >= 0 && index_of(g1, 0) <= V;
+      if (inside) {
+        uint32_t best = key_of(top);
+        for (int j = 0; j < share; ++j) {
+          bound = __reduce_max_sync(~0u, best);
+          if (lane == __ffs(__ballot_sync(~0u, best == bound)) - 1)
+            best = 0;
+        }
+      }
+    } else {
+      bound = 0;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o /= 2) {
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    low = fminf(low, __shfl_xor_sync(~0u, low, o));
+  }
+  if (lane == 0)
+    sh.warp_ends[warp] = Ends{top, low};
+  __syncthreads();
+  if (warp == 0) {
+    top = lane < kWarps ? sh.warp_ends[lane].top : -INFINITY;
+    low = lane < kWarps ? sh.warp_ends[lane].low : INFINITY;
+#pragma unroll
+    for (int o = 16; o; o /= 2) {
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+      low = fminf(low, __shfl_xor_sync(~0u, low, o));
+    }
+    if (lane < ctas)
+      *remote(&sh.ends[rank], lane) = Ends{top, low};
+  }
+  cluster_sync();
+  top = sh.ends[0].top;
+  low = sh.ends[0].low;
+  for (int c = 1; c < ctas; ++c) {
+    top = fmaxf(top, sh.ends[c].top);
+    low = fminf(low, sh.ends[c].low);
+  }
+  if (top == -INFINITY) { // the whole cluster agrees
+    if (rank == 0 && tid == 0) {
+      a.ids[r] = -1;
+      a.prob[r] = 0.f;
+      a.kept[r] = 0;
+    }
+    cluster_sync(); // no CTA leaves while others may still write to it
+    return;
+  }
+
+  // ---- masses and their sums
+  Part own{};
+  {
+    unsigned ones = 0; // masses of 2^32, one short in 32 bits
+    auto add = [&](auto divide, auto bounded) {
+#pragma unroll 1
+      for (int g = g0 + lane; g < g1; g += 32) {
+        const uint4 w = granules[g];
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const float v = at(w, j);
+          const float d = __fsub_rn(top, v);
+          const float e = v == top ? 1.f : expf(-(divide ? __fdiv_rn(d, t) : d));
+          const uint32_t m = __float2uint_rz(e * 4294967296.f);
+          own.all += m;
+          ones += e == 1.f;
+          if (bounded && e >= mp) {
+            own.likely += m + static_cast<u64>(e == 1.f);
+            ++own.likely_n;
+          }
+        }
+      }
+    };
+    struct No { __device__ constexpr operator bool() const { return false; } };
+    struct Yes { __device__ constexpr operator bool() const { return true; } };
+    if (mp > 0.f) {
+      add(Yes{}, Yes{});
+    } else if (t == 1.f) {
+      add(No{}, No{});
+    } else {
+      add(Yes{}, No{});
+    }
+    own.all += ones;
+  }
+  if (mp > 0.f) {
+    own.likely_n = __reduce_add_sync(~0u, own.likely_n);
+    own.likely = warp_sum(own.likely);
+  }
+  own.all = warp_sum(own.all);
+  own.bound = bound;
+  if (lane == 0)
+    sh.warp_part[warp] = own;
+  __syncthreads();
+  if (warp == 0) {
+    Part z{0, 0, 0, 0xFFFFFFFFu};
+    if (lane < kWarps)
+      z = sh.warp_part[lane];
+    own.all = warp_sum(z.all);
+    own.likely = warp_sum(z.likely);
+    own.likely_n = __reduce_add_sync(~0u, z.likely_n);
+    own.bound = __reduce_min_sync(~0u, z.bound);
+    if (lane < ctas)
+      *remote(&sh.part[rank], lane) = own;
+  }
+  cluster_sync();
+  Part sum = sh.part[0];
+  for (int c = 1; c < ctas; ++c) {
+    const Part &y = sh.part[c];
+    sum.all += y.all;
+    sum.likely += y.likely;
+    sum.likely_n += y.likely_n;
+    sum.bound = min(sum.bound, y.bound);
+  }
+
+  // Calls body(x, index) for this warp's logits that pass `test`, each lane
+  // its own ones in turn.
+  auto each_hit = [&](auto test, auto body) {
+    for (int g = g0; g < g1; g += 32 * kGroup) {
+      unsigned hits = 0;
+#pragma unroll
+      for (int q = 0; q < kGroup; ++q) {
+        const int i = g + q * 32 + lane;
+        if (i < g1) {
+          const uint4 w = granules[i];
+#pragma unroll
+          for (int j = 0; j < kVec; ++j)
+            hits |= static_cast<unsigned>(test(at(w, j))) << (q * kVec + j);
+        }
+      }
+      while (hits) {
+        const int b = __ffs(hits) - 1;
+        hits &= hits - 1;
+        const int i = g + b / kVec * 32 + lane;
+        body(one(i, b % kVec), index_of(i, b % kVec));
+      }
+    }
+    __syncwarp();
+  };
+
+  // ---- 2. the bound, as a logit
+  Prefix p{0, V, V, sum.all}; // everything (key 0 is below every logit's)
+  if (k == 1) {
+    p = Prefix{key_of(top), 1, 1, 1ull << 32};
+  } else if (by_k || by_p) {
+    float least = by_k ? value_of(max(sum.bound, key_of(-INFINITY))) : -INFINITY;
+    if (!by_k) {
+      // Shares below this make up less than 1 - p, with a quarter to spare
+      // for the masses' rounding down and this bound's own.
+      const float rest = 0.75f * (1.f - static_cast<float>(p24) * 0x1p-24f) * (__ull2float_rn(sum.all) * 0x1p-32f);
+      const float share = fmaxf(rest / static_cast<float>(V), mp * 0.99f);
+      if (share > 0x1p-31f && share <= 1.f)
+        least = top + t * logf(share) * 1.0001f - 1e-6f * fabsf(top);
+    }
+    least = least == least ? fminf(least, top) : -INFINITY;
+    // ---- 3. histogram over steps of max - x
+    const float reach = fminf(fminf(top - low, kReach * t), top - least);
+    const float steps = reach > 0.f ? kBins / reach : 0.f;
+    auto bin_of = [&](float v) {
+      const float b = v == top ? 0.f : (top - v) * steps; // inf past the last
+      return static_cast<int>(fminf(b, kBins - 1.f));
+    };
+    each_hit([&](float v) { return v >= least; },
+             [&](float v, int) {
+               const int b = bin_of(v);
+               const u64 w = mass_of(share_of(v, top, t));
+               atomicAdd(&sh.bins.count[b], 1u);
+               // 16 bits at a time: at most 2^15 logits of a CTA a step carry
+               // mass (the launcher's bound on a run), no carry is lost.
+               if (w) {
+                 atomicAdd(&sh.bins.lo[b], static_cast<unsigned>(w) & 0xFFFFu);
+                 atomicAdd(&sh.bins.hi[b], static_cast<unsigned>(w >> 16));
+               }
+             });
+    cluster_sync();
+    // Every CTA sums and scans all of it: two neighbouring steps a thread.
+    u64 mass[2] = {0, 0};
+    int count[2] = {0, 0};
+    if (2 * tid < kBins) {
+      for (int c = 0; c < ctas; ++c) {
+        const auto *h = remote(&sh.bins, c);
+        const uint2 n2 = *reinterpret_cast<const uint2 *>(h->count + 2 * tid);
+        const uint2 l2 = *reinterpret_cast<const uint2 *>(h->lo + 2 * tid);
+        const uint2 h2 = *reinterpret_cast<const uint2 *>(h->hi + 2 * tid);
+        count[0] += static_cast<int>(n2.x);
+        count[1] += static_cast<int>(n2.y);
+        mass[0] += l2.x + (static_cast<u64>(h2.x) << 16);
+        mass[1] += l2.y + (static_cast<u64>(h2.y) << 16);
+      }
+    }
+    u64 m0 = mass[0] + mass[1], m_total;
+    int n0 = count[0] + count[1], n_total;
+    block_scan(m0, n0, sh, m_total, n_total);
+    bool drained = false; // whether every CTA has read the bins
+    auto end_in = [&](bool by_mass, u64 want) {
+      if (by_mass && m_total < want) // min-p ends it before p does
+        return Prefix{0, V, INT_MAX, sum.all};
+      {
+        u64 mm = m0;
+        int nn = n0;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const bool here = by_mass ? mm < want && mm + mass[q] >= want
+                                    : nn < static_cast<int>(want) && nn + count[q] >= static_cast<int>(want);
+          if (here) {
+            sh.edge_bin = 2 * tid + q;
+            sh.edge_count = count[q];
+            sh.edge_before = nn;
+            sh.edge_mass = mm;
+          }
+          mm += mass[q];
+          nn += count[q];
+        }
+      }
+      __syncthreads();
+      const int b = sh.edge_bin, n_in = sh.edge_count, n_before = sh.edge_before;
+      const u64 m_before = sh.edge_mass;
+      if (n_in > kCap) { // ---- 4. too many near each other
+        if (!drained)
+          cluster_sync(); // the digit search takes the bins' place
+        drained = true;
+        return select<TYPE>(row, V, top, t, by_mass, want, sh.digits);
+      }
+      // Every CTA gets all logits of the step.
+      const int slot = by_mass;
+      each_hit([&](float v) { return v >= least && bin_of(v) == b; },
+               [&](float v, int i) {
+                 const u64 key = static_cast<u64>(key_of(v)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(i));
+                 for (int c = 0; c < ctas; ++c)
+                   remote(&sh.keys[slot][0], c)[atomicAdd(remote(&sh.taken[slot], c), 1)] = key;
+               });
+      cluster_sync();
+      drained = true;
+      return resolve(sh, sh.keys[slot], n_in, n_before, m_before, by_mass, want, top, t);
+    };
+    if (by_k)
+      p = end_in(false, k);
+    if (by_p)
+      p = end_in(true, max(part_of(p.mass, p24), 1ull));
+  }
+  const bool few = mp > 0.f && sum.likely_n < p.count; // min-p ends it earlier
+  const u64 mass = few ? sum.likely : p.mass;
+  const int kept = few ? sum.likely_n : p.count;
+
+  // ---- 5. the draw
+  const u64 target = part_of(mass, u24);
+  const float edge = p.key ? value_of(p.key) : -INFINITY;
+  const u64 each = p.key ? mass_of(share_of(edge, top, t)) : 0;
+  // Mass of one logit that stays for sure; 0 for those equal to the edge.
+  auto sure = [&](float v) {
+    const float e = share_of(v, top, t);
+    return e >= mp && (p.key == 0 || v > edge) ? mass_of(e) : 0ull;
+  };
+  const bool edge_passes = p.key && share_of(edge, top, t) >= mp;
+  u64 mine = 0;
+  int ties = 0;
+  each_hit([&](float v) { return v >= edge && v > -INFINITY; },
+           [&](float v, int) {
+             mine += sure(v);
+             ties += edge_passes && v == edge;
+           });
+  mine = warp_sum(mine);
+  ties = __reduce_add_sync(~0u, ties);
+  if (lane == 0) {
+    sh.warp[warp] = mine;
+    sh.warp_n[warp] = ties;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const u64 m = warp_sum(lane < kWarps ? sh.warp[lane] : 0);
+    const int n = __reduce_add_sync(~0u, lane < kWarps ? sh.warp_n[lane] : 0);
+    if (lane < ctas) {
+      *remote(&sh.drawn[rank], lane) = m;
+      *remote(&sh.tied[rank], lane) = n;
+    }
+  }
+  cluster_sync(); // the last exchange
+  // What stays before this warp's run: the sure ones, and of those equal to
+  // the edge the first p.ties by index.
+  u64 before = 0;
+  int tied = 0;
+  for (int c = 0; c < rank; ++c) {
+    before += sh.drawn[c];
+    tied += sh.tied[c];
+  }
+  for (int w = 0; w < warp; ++w) {
+    before += sh.warp[w];
+    tied += sh.warp_n[w];
+  }
+  const u64 start = before + each * min(tied, p.ties), end = before + mine + each * min(tied + ties, p.ties);
+  if (!(start <= target && target < end))
+    return;
+  // This warp's run holds the token.
+  u64 cum = start;
+  for (int g = g0; g < g1; g += 32) {
+    const int i = g + lane;
+    u64 m[kVec], sum_m = 0;
+    const uint4 w = i < g1 ? granules[i] : make_uint4(0, 0, 0, 0);
+    int equal = 0;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+      equal += i < g1 && edge_passes && at(w, j) == edge;
+    const int equal_run = warp_scan(equal);
+    int rank_of = tied + equal_run - equal;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const float v = at(w, j);
+      m[j] = i < g1 && v >= edge && v > -INFINITY ? sure(v) : 0;
+      if (i < g1 && edge_passes && v == edge)
+        m[j] = rank_of++ < p.ties ? each : 0;
+      sum_m += m[j];
+    }
+    const u64 run = warp_scan(sum_m);
+    const unsigned past = __ballot_sync(~0u, cum + run > target);
+    if (past) {
+      if (lane == __ffs(past) - 1) {
+        u64 c = cum + run - sum_m;
+        bool found = false;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          c += m[j];
+          if (!found && c > target) {
+            found = true;
+            a.ids[r] = index_of(i, j);
+            a.prob[r] = __fdiv_rn(__ull2float_rn(m[j]), __ull2float_rn(sum.all));
+            a.kept[r] = kept;
+          }
+        }
+      }
+      return;
+    }
+    cum += __shfl_sync(~0u, run, 31);
+    tied += __shfl_sync(~0u, equal_run, 31);
+  }
+}
+
+template <int TYPE> cudaError_t sample_type(const SampleArgs &a, cudaStream_t stream) {
+  constexpr int kVec = TYPE == LOGIT_F32 ? 4 : 8;
+  // Granules of 16 bytes that a row may touch; a CTA's run has at most 2^15
+  // logits (the histogram's sums).
+  const int granules = a.vocab / kVec + 2;
+  constexpr int kMost = (1 << 15) / kVec;
+  if (granules > kMostCtas * kMost)
+    return launch_pdl(sample_long_kernel<TYPE>, a.rows, kThreads, 0, stream, a);
+  // CTAs per row: while all rows fit the GPU at once (three an SM) and a CTA
+  // has 2048 logits or more, spread them; then as many as a row needs.
+  int ctas = 1;
+  while (ctas < kMostCtas && a.rows * 2ll * ctas <= 3ll * sm_count() && granules > ctas * 4096 / kVec)
+    ctas *= 2;
+  while (ctas < kMostCtas && granules > ctas * kMost)
+    ctas *= 2;
+  auto *kernel = sample_row_kernel<TYPE>;
+  const int smem = (granules + ctas - 1) / ctas * 16;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost * 16);
+  if (e != cudaSuccess)
+    return e;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = kRowThreads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  for (int r = 0; r < a.rows; r += 65535) {
+    SampleArgs b = a;
+    b.rows = std::min(a.rows - r, 65535);
+    b.logits = static_cast<const char *>(a.logits) + r * a.stride * (16 / kVec);
+    b.temperature = a.temperature ? a.temperature + r : nullptr;
+    b.top_k = a.top_k ? a.top_k + r : nullptr;
+    b.top_p = a.top_p ? a.top_p + r : nullptr;
+    b.min_p = a.min_p ? a.min_p + r : nullptr;
+    b.uniform = a.uniform + r;
+    b.ids = a.ids + r;
+    b.prob = a.prob + r;
+    b.kept = a.kept + r;
+    cfg.gridDim = dim3(ctas, b.rows);
+    e = cudaLaunchKernelEx(&cfg, kernel, b);
+    if (e != cudaSuccess)
+      return e;
+  }
+  return cudaSuccess;
+}
+
 } // namespace
 
 cudaError_t sample_tokens(const SampleArgs &a, int type, cudaStream_t stream) {
-  auto *kernel = type == LOGIT_F32    ? sample_kernel<LOGIT_F32>
-                 : type == LOGIT_BF16 ? sample_kernel<LOGIT_BF16>
-                                      : sample_kernel<LOGIT_F16>;
-  return launch_pdl(kernel, a.rows, kThreads, 0, stream, a);
+  switch (type) {
+  case LOGIT_F32: return sample_type<LOGIT_F32>(a, stream);
+  case LOGIT_BF16: return sample_type<LOGIT_BF16>(a, stream);
+  case LOGIT_F16: return sample_type<LOGIT_F16>(a, stream);
+  }
+  return cudaErrorInvalidValue;
 }
 
 } // namespace pb2

@@ -552,6 +552,19 @@ def test_sample_per_row_parameters_and_strides(native, cuda):
         assert (int(one[0][0]), float(one[1][0]), int(one[2][0])) == (int(ids[r]), float(prob[r]), int(kept[r]))
 
 
+@pytest.mark.parametrize("vocab", [300, 9000, 60000, 170000])
+@pytest.mark.parametrize("kw", [{"top_p": 0.99}, {"top_p": 0.7, "temperature": 4.0}, {"top_k": 5000},
+                                {"top_k": 5000, "top_p": 0.9}, {"top_p": 0.9999, "min_p": 1e-4}])
+def test_sample_flat_distributions(native, cuda, vocab, kw):
+    """Prefixes of thousands of tokens: beyond what is sorted at once."""
+    x, u = logits_of(4, vocab, vocab, F16 if vocab < 1000 else torch.float32, std=1.0)
+    x[1] = torch.randn(vocab, generator=gen(77)).to(x.dtype) * 0.01
+    x[2] = torch.round(x[2].float() * 2).to(x.dtype) / 2      # few distinct values
+    x[3, : vocab // 2] = -math.inf
+    check_sample(x, u, **kw)
+    assert fault(native) == 0
+
+
 def test_sample_frequencies(native, cuda):
     """Evenly spread uniform numbers hit every token as often as its share."""
     x = torch.tensor([[0.0, 1.0, 2.0, -1.0, 3.0]]).expand(4096, 5).contiguous()
