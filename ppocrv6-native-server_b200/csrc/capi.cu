@@ -798,8 +798,9 @@ int ppocr_b200_kv4_attention(const PpocrKv4Cache *cache, const void *q, long lon
     return fail(std::string("kv4 attention: ") + bad);
   if (heads <= 0 || heads % c.kv_heads)
     return fail("kv4 attention: heads must be a multiple of kv_heads");
-  if (static_cast<long long>(max_new) * (heads / c.kv_heads) >= (1ll << 30))
-    return fail("kv4 attention: max_new * heads / kv_heads is too large");
+  if (static_cast<long long>(max_new) * (heads / c.kv_heads) >= (1ll << 30) ||
+      static_cast<long long>(max_new) * heads / 256 * batch >= (1ll << 30))
+    return fail("kv4 attention: batch * max_new * heads is too large");
   if (window < 0 || sinks < 0 || !(scale - scale == 0.f))
     return fail("kv4 attention: window and sinks must not be negative, scale must be finite");
   if (batch == 0 || tokens == 0 || max_new == 0)
@@ -818,7 +819,8 @@ int ppocr_b200_kv4_attention(const PpocrKv4Cache *cache, const void *q, long lon
   a.sinks = sinks;
   a.scale = scale;
   a.workspace = workspace;
-  return status(kv4_attend_rows(c, t, a, stream), "kv4 attention");
+  const long long rows = static_cast<long long>(max_new) * (heads / c.kv_heads);
+  return status(rows <= 32 ? kv4_attend_rows(c, t, a, stream) : kv4_attend_prompt(c, t, a, stream), "kv4 attention");
 }
 
 int ppocr_b200_sample(const void *logits, int type, long long stride, int rows, int vocab, const float *temperature,

@@ -384,6 +384,8 @@ struct Kv4Attention {
   void *workspace = nullptr;
 };
 cudaError_t kv4_attend_rows(const Kv4Cache &c, const Kv4Tokens &t, const Kv4Attention &a, cudaStream_t stream);
+// The same with many query rows, on tcgen05.
+cudaError_t kv4_attend_prompt(const Kv4Cache &c, const Kv4Tokens &t, const Kv4Attention &a, cudaStream_t stream);
 // Token sampling (csrc/sample.cu); the parameters are per row, null = off.
 struct SampleArgs {
   const void *logits = nullptr;

@@ -1,0 +1,528 @@
+// Attention over the 4-bit cache for prompts and chunks (many query rows per
+// (sequence, key head)), on the tensor cores (tcgen05 + TMEM).
+//
+// A CTA owns 256 query rows of one (sequence, key head): rows are (token,
+// head of the group) pairs, so the heads that share a key head share its
+// restored keys and values. It walks the 128-key tiles that its rows see:
+//  * four warps restore the tile from the cache's pages (two codes a byte,
+//    scale * c + minimum rounded once to the cache's 16-bit type) into shared
+//    memory, keys and values alike as rows of a token, 128-byte swizzled; the
+//    next tile's codes are in registers by then;
+//  * one thread issues S = Q K^T for two blocks of 128 rows (K is K-major)
+//    and O += P V (V as it lies is the MN-major operand, P comes from TMEM);
+//  * four warps per block of rows, one row a thread, turn S into P in place:
+//    the fp32 score's columns become 16-bit probabilities in the first half
+//    of the same TMEM columns. The running maximum is only raised when a score
+//    passes it by more than 8 (in powers of two), so O in TMEM is rescaled
+//    rarely; while one block's rows are in the softmax, the other's products
+//    run.
+// Products are issued in the order P0 V(j), S0(j + 1), P1 V(j), S1(j + 1): a
+// commit after S t (j + 1) also says that O t holds all of tile j.
+// Work per tile: 4 x 128 x 128 x D multiply-adds (2048 cycles of the tensor
+// pipe at D = 128) against 32768 exponentials (2048 cycles of the special
+// function units): the two bound it alike.
+#include "kv4.cuh"
+#include <algorithm>
+
+namespace pb2 {
+namespace {
+
+constexpr int kPromptThreads = 13 * 32; // 2 x 4 softmax warps, 4 restoring, 1 issuing
+constexpr int kTile = 128;
+constexpr int kBlockRows = 256;
+constexpr uint32_t kAtom = 128 * 128; // 128 rows of 128 bytes
+constexpr int kErrPromptWait = 43;
+
+struct PromptArgs {
+  Kv4Tokens t;
+  const uint8_t *pool;
+  const uint16_t *q;
+  uint16_t *out;
+  long long q_stride;
+  int heads, kv_heads, group;
+  int window, sinks;
+  float scale_log2; // |softmax scale| * log2(e)
+  uint32_t flip;    // sign of the scale, as a mask of two 16-bit values
+  int row_blocks;
+  FastDiv group_div, unit_div, heads_div; // by group, batch * kv_heads, kv_heads
+};
+
+template <int D> struct PromptLayout {
+  static constexpr int kAtoms = D > 64 ? 2 : 1; // 64-channel columns
+  static constexpr uint32_t kOperand = kAtoms * kAtom;
+  static constexpr uint32_t kOffQ = 0;
+  static constexpr uint32_t kOffK = 2 * kOperand;
+  static constexpr uint32_t kOffV = 4 * kOperand;
+  static constexpr uint32_t kOffBars = 6 * kOperand;
+  static constexpr size_t kBytes = kOffBars + 256 + 1024;
+};
+
+// D[tmem] (+)= A[tmem] * B[smem desc], 16-bit inputs, fp32 accumulator.
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t"
+               "setp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+               "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+// Descriptor of an MN-major operand: rows of 64 values of the MN dimension
+// (128 bytes, swizzled), 8 K rows per 1024-byte atom; the next 64 values of
+// the MN dimension one operand column further.
+__device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(kAtom >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                 "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+                 "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+                 "=r"(r[30]), "=r"(r[31])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+               "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+               "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+               "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+               "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+               "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+               "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+               "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Eight channels of one token from their codes: packed values in order.
+template <bool BF16> __device__ __forceinline__ uint4 restore_row(uint32_t w, uint32_t scale, uint32_t low) {
+  uint32_t v[4]; // channels (0,4), (1,5), (2,6), (3,7)
+  if constexpr (BF16) {
+    const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162 *>(&scale);
+    const __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162 *>(&low);
+    const uint32_t off = 0x43004300u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u; // 128 + c
+      const __nv_bfloat162 r = __hfma2(
+          __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&c), *reinterpret_cast<const __nv_bfloat162 *>(&off)), s, m);
+      v[i] = *reinterpret_cast<const uint32_t *>(&r);
+    }
+  } else {
+    const __half2 s = *reinterpret_cast<const __half2 *>(&scale);
+    const __half2 m = *reinterpret_cast<const __half2 *>(&low);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t y = i < 2 ? w : w >> 8;
+      const uint32_t c = (y & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u; // 1024 + c or 1024 + 16 c
+      const __half2 x = *reinterpret_cast<const __half2 *>(&c);
+      const __half2 n = i & 1 ? __hfma2(x, __float2half2_rn(0.0625f), __float2half2_rn(-64.f))
+                              : __hsub2(x, __float2half2_rn(1024.f));
+      const __half2 r = __hfma2(n, s, m);
+      v[i] = *reinterpret_cast<const uint32_t *>(&r);
+    }
+  }
+  return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
+                    __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs g) {
+  using L = PromptLayout<D>;
+  constexpr int G = D / 32;
+  extern __shared__ uint8_t prompt_smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(prompt_smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kOffBars);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7;
+  uint64_t *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 13, *drain = bars + 15;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16);
+  volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(q_full, 256);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full + i, 128);
+      mbar_init(v_full + i, 128);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 128);
+      mbar_init(o_full + i, 1);
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    fence_barrier_init();
+  }
+  // All of TMEM is taken only after the kernels before have ended, and the
+  // next kernel is let in only after it is taken: neither side can hold
+  // columns that the other's unfinished CTAs wait for.
+  pdl_wait();
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  const uint32_t tmem = *tmem_slot;
+
+  // Last rows first: they see the most keys.
+  const uint32_t slab = g.unit_div.div(blockIdx.x);
+  const uint32_t unit = blockIdx.x - slab * (g.t.batch * g.kv_heads);
+  const int b = g.heads_div.div(unit), h = unit - b * g.kv_heads;
+  const int row0 = (g.row_blocks - 1 - static_cast<int>(slab)) * kBlockRows;
+  const Kv4Seq seq = kv4_seq(g.t, b);
+  const int rows = min(seq.n * g.group - row0, kBlockRows);
+  const int past = seq.len - seq.n;
+  // The key tiles that these rows see: [0, sink) and [lo, hi).
+  int sink = 0, lo = 0, tiles = 0;
+  int pos_lo = 0, pos_hi = -1;
+  if (rows > 0) {
+    pos_lo = past + static_cast<int>(g.group_div.div(row0));
+    pos_hi = past + static_cast<int>(g.group_div.div(row0 + rows - 1));
+    const int hi = max((pos_hi + kTile) / kTile, 1);
+    if (g.window > 0) {
+      const int first = max(pos_lo + 1 - g.window, 0);
+      lo = first / kTile;
+      sink = (min(g.sinks, first) + kTile - 1) / kTile;
+      if (sink >= lo)
+        sink = lo = 0;
+    }
+    tiles = sink + hi - lo;
+  }
+  const bool two = rows > 128;
+  auto key_of_tile = [&](int j) { return (j < sink ? j : j - sink + lo) * kTile; };
+  bool ok = true;
+
+  if (tiles > 0 && warp < 8) {
+    // ------------------------------------------------------------- softmax
+    const int block = warp >> 2;
+    const int row = tid & 127; // within the block of 128
+    const int r = block * 128 + row;
+    const bool live = r < rows;
+    const uint32_t i = g.group_div.div(row0 + r);
+    const int head = h * g.group + static_cast<int>(row0 + r - i * g.group);
+    const int pos = live ? past + static_cast<int>(i) : -1;
+    {
+      const uint4 *src =
+          reinterpret_cast<const uint4 *>(g.q + (seq.first + static_cast<long long>(i)) * g.q_stride + head * D);
+      const uint32_t dst = sbase + L::kOffQ + block * L::kOperand + row * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 w = live ? src[c] : make_uint4(0, 0, 0, 0);
+        w.x ^= g.flip, w.y ^= g.flip, w.z ^= g.flip, w.w ^= g.flip;
+        sts_v4(dst + (c / 8) * kAtom + (((c & 7) ^ (row & 7)) << 4), w);
+      }
+      fence_async_smem();
+      mbar_arrive(q_full);
+    }
+    if (block == 0 || two) {
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t t_s = tmem + lanes + block * 128, t_o = tmem + lanes + 256 + block * 128;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < tiles; ++j) {
+        ok = mbar_wait(s_full + block, j & 1, abort);
+        ok = __all_sync(~0u, ok);
+        if (!ok)
+          break;
+        tc_fence_after();
+        const int key0 = key_of_tile(j);
+        const bool clear = key0 + kTile - 1 <= pos_lo &&
+                           (g.window <= 0 || key0 > pos_hi - g.window || key0 + kTile <= g.sinks);
+        // Key offsets that this row sees: [0, to) without a window, and with
+        // one those at or past `from` or below `first`.
+        const int to = pos - key0, from = g.window > 0 ? to - g.window : -1, first = g.sinks - key0;
+        auto seen = [&](int c) { return c <= to && (c > from || c < first); };
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t s[32];
+          tmem_ld32(t_s + 32 * c, s);
+          tmem_ld_wait();
+          if (clear) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              top = fmaxf(top, __uint_as_float(s[e]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              top = fmaxf(top, seen(32 * c + e) ? __uint_as_float(s[e]) : -INFINITY);
+          }
+        }
+        const float up = fmaxf(m, top * g.scale_log2);
+        if (__any_sync(~0u, up > m + 8.f)) {
+          const float f = up > m ? ex2_ftz(m - up) : 1.f;
+          m = up;
+          l *= f;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(t_o + 32 * c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(t_o + 32 * c, o);
+            }
+          }
+        }
+        const float minus = m == -INFINITY ? 0.f : -m;
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t s[32], p[16];
+          tmem_ld32(t_s + 32 * c, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float2 x = make_float2(minus, minus);
+            ffma2(x, make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
+                  make_float2(g.scale_log2, g.scale_log2));
+            if (!clear) {
+              x.x = seen(32 * c + e) ? x.x : -INFINITY;
+              x.y = seen(32 * c + e + 1) ? x.y : -INFINITY;
+            }
+            x.x = ex2_ftz(x.x);
+            x.y = ex2_ftz(x.y);
+            sum.x += x.x;
+            sum.y += x.y;
+            p[e / 2] = kv4_pack<BF16>(x.x, x.y);
+          }
+          tmem_st16(t_s + 16 * c, p);
+        }
+        l += sum.x + sum.y;
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(p_full + block);
+      }
+      if (ok) {
+        ok = mbar_wait(o_full + block, 0, abort);
+        ok = __all_sync(~0u, ok);
+      }
+      if (ok) {
+        tc_fence_after();
+        const float f = l > 0.f ? __fdividef(1.f, l) : l; // nothing seen: 0; NaN stays NaN
+        uint16_t *dst = g.out + ((seq.first + static_cast<long long>(i)) * g.heads + head) * D;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + 32 * c, o);
+          tmem_ld_wait();
+          if (live)
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 w;
+              w.x = kv4_pack<BF16>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
+              w.y = kv4_pack<BF16>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
+              w.z = kv4_pack<BF16>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
+              w.w = kv4_pack<BF16>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
+              *reinterpret_cast<uint4 *>(dst + 32 * c + e) = w;
+            }
+        }
+      }
+    }
+  } else if (tiles > 0 && warp < 12) {
+    // ----------------------------------------------------------- restoring
+    const int w = tid - 256;
+    constexpr int kPer = 128 / G; // tokens a pass
+    const int page = 1 << g.t.page_shift;
+    const int tok0 = w / G, c = w % G; // token of the pass, group
+    uint4 kc[G], vc[G];
+    uint32_t kp[G], vp[G];
+    auto fetch = [&](int j) {
+      const int key0 = key_of_tile(j);
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int key = key0 + i * kPer + tok0;
+        kc[i] = vc[i] = make_uint4(0, 0, 0, 0);
+        kp[i] = vp[i] = 0; // past the length: zeros
+        if (key < seq.len) {
+          const long long p = kv4_page(g.t, b, key);
+          const int slot = key & (page - 1);
+          const uint8_t *blk = g.pool + (p * g.kv_heads + h) * static_cast<long long>(page * (D + D / 4));
+          const uint8_t *codes = blk + slot * (D / 2) + c * 16;
+          const uint8_t *params = blk + page * D + slot * (D / 8) + c * 4;
+          kc[i] = __ldg(reinterpret_cast<const uint4 *>(codes));
+          vc[i] = __ldg(reinterpret_cast<const uint4 *>(codes + page * (D / 2)));
+          kp[i] = __ldg(reinterpret_cast<const uint32_t *>(params));
+          vp[i] = __ldg(reinterpret_cast<const uint32_t *>(params + page * (D / 8)));
+        }
+      }
+    };
+    auto put = [&](uint32_t base, const uint4 (&codes)[G], const uint32_t (&params)[G]) {
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int tok = i * kPer + tok0;
+        const uint32_t scale = __byte_perm(params[i], 0, 0x1010), low = __byte_perm(params[i], 0, 0x3232);
+        // Lanes of the upper two groups write their chunks in another order,
+        // so that the eight lanes of a phase meet eight bank columns.
+        const bool turn = c >= 2;
+        const uint32_t in[4] = {turn ? codes[i].z : codes[i].x, turn ? codes[i].w : codes[i].y,
+                                turn ? codes[i].x : codes[i].z, turn ? codes[i].y : codes[i].w};
+        const uint32_t row = base + (c / 2) * kAtom + tok * 128;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int chunk = (c & 1) * 4 + (turn ? e ^ 2 : e);
+          sts_v4(row + ((chunk ^ (tok & 7)) << 4), restore_row<BF16>(in[e], scale, low));
+        }
+      }
+    };
+    fetch(0);
+    for (int j = 0; j < tiles; ++j) {
+      const int st = j & 1;
+      if (j >= 2) {
+        ok = mbar_wait(k_empty + st, (j / 2 - 1) & 1, abort);
+        ok = __all_sync(~0u, ok);
+        if (!ok)
+          break;
+      }
+      put(sbase + L::kOffK + st * L::kOperand, kc, kp);
+      fence_async_smem();
+      mbar_arrive(k_full + st);
+      if (j >= 2) {
+        ok = mbar_wait(v_empty + st, (j / 2 - 1) & 1, abort);
+        ok = __all_sync(~0u, ok);
+        if (!ok)
+          break;
+      }
+      put(sbase + L::kOffV + st * L::kOperand, vc, vp);
+      fence_async_smem();
+      mbar_arrive(v_full + st);
+      if (j + 1 < tiles)
+        fetch(j + 1);
+    }
+  } else if (tiles > 0 && lane == 0) {
+    // ------------------------------------------------------------- issuing
+    constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
+    constexpr uint32_t idesc_s = idesc_f16_f32(128, 128) | kType;
+    constexpr uint32_t idesc_o = idesc_f16_f32(128, D) | kType | (1u << 16); // B is MN-major
+    auto scores = [&](int block, int st) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t off = (k / 4) * kAtom + (k & 3) * 32;
+        umma_f16(tmem + block * 128, sdesc_k_sw128(sbase + L::kOffQ + block * L::kOperand + off),
+                 sdesc_k_sw128(sbase + L::kOffK + st * L::kOperand + off), idesc_s, k != 0);
+      }
+      umma_commit(s_full + block);
+    };
+    auto values = [&](int block, int st, int j) {
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k)
+        umma_ts(tmem + 256 + block * 128, tmem + block * 128 + k * 8,
+                sdesc_mn_sw128(sbase + L::kOffV + st * L::kOperand + k * 2048), idesc_o, j != 0 || k != 0);
+    };
+    ok = mbar_wait(q_full, 0, abort) && mbar_wait(k_full, 0, abort);
+    if (ok) {
+      tc_fence_after();
+      scores(0, 0);
+      if (two)
+        scores(1, 0);
+      umma_commit(k_empty);
+    }
+    for (int j = 0; ok && j < tiles; ++j) {
+      const int st = j & 1, next = st ^ 1;
+      const bool more = j + 1 < tiles;
+      ok = mbar_wait(v_full + st, (j / 2) & 1, abort) && (!more || mbar_wait(k_full + next, ((j + 1) / 2) & 1, abort));
+      for (int block = 0; ok && block < (two ? 2 : 1); ++block) {
+        ok = mbar_wait(p_full + block, j & 1, abort);
+        if (!ok)
+          break;
+        tc_fence_after();
+        values(block, st, j);
+        if (more)
+          scores(block, next);
+        else
+          umma_commit(o_full + block);
+      }
+      if (ok) {
+        umma_commit(v_empty + st);
+        if (more)
+          umma_commit(k_empty + next);
+      }
+    }
+    if (!ok) {
+      // Everything issued ends before the memory goes away.
+      *abort = 1;
+      umma_commit(drain);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(drain, 0) && clock64() - t0 < kWaitBudgetCycles) {
+      }
+    }
+  }
+  if (!ok) {
+    *abort = 1;
+    if (lane == 0)
+      kv4_fault(g.t, kErrPromptWait);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0)
+    tmem_dealloc(tmem, 512);
+}
+
+template <int D, bool BF16> cudaError_t launch_prompt(const PromptArgs &g, cudaStream_t stream) {
+  auto *kernel = prompt_kernel<D, BF16>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(PromptLayout<D>::kBytes));
+  if (e != cudaSuccess)
+    return e;
+  const unsigned grid = static_cast<unsigned>(g.row_blocks) * g.t.batch * g.kv_heads;
+  return launch_pdl(kernel, grid, kPromptThreads, PromptLayout<D>::kBytes, stream, g);
+}
+
+} // namespace
+
+cudaError_t kv4_attend_prompt(const Kv4Cache &c, const Kv4Tokens &t, const Kv4Attention &a, cudaStream_t stream) {
+  PromptArgs g{};
+  g.t = t;
+  g.pool = c.pool;
+  g.q = static_cast<const uint16_t *>(a.q);
+  g.out = static_cast<uint16_t *>(a.out);
+  g.q_stride = a.q_stride;
+  g.heads = a.heads;
+  g.kv_heads = c.kv_heads;
+  g.group = a.heads / c.kv_heads;
+  g.window = a.window;
+  g.sinks = a.sinks;
+  g.scale_log2 = fabsf(a.scale) * kLog2e;
+  g.flip = a.scale < 0.f ? 0x80008000u : 0u;
+  const long long blocks = (static_cast<long long>(t.max_new) * g.group + kBlockRows - 1) / kBlockRows;
+  // Block indices are divided in 31 bits.
+  if (blocks * t.batch * c.kv_heads >= (1ll << 31))
+    return cudaErrorInvalidValue;
+  g.row_blocks = static_cast<int>(blocks);
+  g.group_div = FastDiv(g.group);
+  g.unit_div = FastDiv(t.batch * c.kv_heads);
+  g.heads_div = FastDiv(c.kv_heads);
+  switch (c.head_dim * 2 + c.bf16) {
+  case 64: return launch_prompt<32, false>(g, stream);
+  case 65: return launch_prompt<32, true>(g, stream);
+  case 128: return launch_prompt<64, false>(g, stream);
+  case 129: return launch_prompt<64, true>(g, stream);
+  case 256: return launch_prompt<128, false>(g, stream);
+  case 257: return launch_prompt<128, true>(g, stream);
+  }
+  return cudaErrorInvalidValue;
+}
+
+} // namespace pb2

@@ -31,7 +31,8 @@ COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
 
 LIB_SOURCES = ["common.cu", "tc_gemm.cu", "halo_conv.cu", "dwpw.cu", "stem_tc.cu", "spatial.cu", "seq.cu", "head.cu",
                "detect.cu", "components.cu", "preprocess.cu", "lines.cu", "runtime.cu", "capi.cu",
-               "head_noalloc.cu", "attention_tc.cu", "matmul_tc.cu", "kv4_cache.cu", "kv4_rows.cu", "sample.cu"]
+               "head_noalloc.cu", "attention_tc.cu", "matmul_tc.cu", "kv4_cache.cu", "kv4_rows.cu", "kv4_prompt.cu",
+               "sample.cu"]
 
 
 def _run(cmd: list[str]) -> None:

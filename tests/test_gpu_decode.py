@@ -276,6 +276,50 @@ def test_attention_few_tokens(native, cuda, new, lengths, heads, kv, dim, page, 
     check_attention(native, s, heads, window=window, sinks=sinks, keys_rounded=True)
 
 
+PROMPT_CASES = [
+    # new, lengths, heads, kv heads, dim, page, type
+    ([33], [33], 1, 1, 64, 16, F16),
+    ([128], [128], 1, 1, 128, 128, F16),
+    ([129], [129], 1, 1, 128, 64, BF16),
+    ([1, 64, 0, 127], [1, 64, 0, 127], 2, 2, 32, 16, F16),
+    ([256, 257, 90], [256, 257, 400], 4, 4, 64, 32, BF16),
+    ([70, 300], [700, 1500], 8, 2, 128, 64, F16),
+    ([100], [1000], 16, 1, 32, 128, BF16),
+    ([65, 8], [2000, 9], 12, 4, 128, 16, BF16),
+    ([700], [700], 6, 2, 64, 64, F16),
+]
+
+
+@pytest.mark.parametrize("new,lengths,heads,kv,dim,page,dtype", PROMPT_CASES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 0), (300, 9)])
+def test_attention_prompt(native, cuda, new, lengths, heads, kv, dim, page, dtype, window, sinks):
+    s = Scene(lengths, new, kv, dim, page, dtype, seed=sum(lengths) + dim)
+    some = {0, 1, 15, 16, 31, 32, 63, 64, 65, 127, 128, 129, 255, 256, 300}
+    check_attention(native, s, heads, window=window, sinks=sinks, keys_rounded=True, rows=some)
+
+
+@pytest.mark.parametrize("scale", [4.0, -0.1, 0.0])
+def test_attention_prompt_scales(native, cuda, scale):
+    s = Scene([400], [200], 2, 128, 32, F16, seed=41)
+    check_attention(native, s, 4, scale=scale, keys_rounded=True, rows={0, 100, 150})
+
+
+def test_attention_prompt_nan_stays_in_its_row(native, cuda):
+    s = Scene([300], [100], 2, 64, 16, F16, seed=42)
+    s.fill([300])
+    cache = s.cache()
+    table, lens = s.places()
+    q = torch.randn(100, 4, 64, generator=gen(3)).half()
+    clean = cache.attention(q.cuda(), table, lens)
+    q[40, 1, 7] = math.nan
+    got = cache.attention(q.cuda(), table, lens)
+    assert fault(native) == 0
+    assert torch.isnan(got[40, 1].float()).all()
+    keep = torch.ones(100, 4, dtype=torch.bool)
+    keep[40, 1] = False
+    assert torch.equal(got.cpu()[keep], clean.cpu()[keep])
+
+
 def test_attention_large_scores(native, cuda):
     """Scores far beyond exp's range: the running maximum carries them."""
     s = Scene([600, 70], [1, 1], 2, 128, 32, F16, seed=3)
