@@ -4,10 +4,12 @@
 // A CTA owns 256 query rows of one (sequence, key head): rows are (token,
 // head of the group) pairs, so the heads that share a key head share its
 // restored keys and values. It walks the 128-key tiles that its rows see:
-//  * four warps restore the tile from the cache's pages (two codes a byte,
-//    scale * c + minimum rounded once to the cache's 16-bit type) into shared
-//    memory, keys and values alike as rows of a token, 128-byte swizzled; the
-//    next tile's codes are in registers by then;
+//  * four warps restore the tile's keys and four its values from the cache's
+//    pages (two codes a byte, scale * c + minimum rounded once to the cache's
+//    16-bit type) into shared memory, as rows of a token, 128-byte swizzled;
+//    the next tile's codes are in registers and the page ids of the one after
+//    by then. Channels lie in the order 0 4 1 5 2 6 3 7 of every eight, as the
+//    codes' masks give them: queries are reordered alike, the output back;
 //  * one thread issues S = Q K^T for two blocks of 128 rows (K is K-major)
 //    and O += P V (V as it lies is the MN-major operand, P comes from TMEM);
 //  * four warps per block of rows, one row a thread, turn S into P in place:
@@ -23,11 +25,12 @@
 // function units): the two bound it alike.
 #include "kv4.cuh"
 #include <algorithm>
+#include <type_traits>
 
 namespace pb2 {
 namespace {
 
-constexpr int kPromptThreads = 13 * 32; // 2 x 4 softmax warps, 4 restoring, 1 issuing
+constexpr int kPromptThreads = 17 * 32; // 2 x 4 softmax warps, 2 x 4 restoring, 1 issuing
 constexpr int kTile = 128;
 constexpr int kBlockRows = 256;
 constexpr uint32_t kAtom = 128 * 128; // 128 rows of 128 bytes
@@ -109,9 +112,23 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Eight channels of one token from their codes: packed values in order.
+// The 16-bit values of a 16-byte chunk in the order 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ uint4 interleave(uint4 w) {
+  return make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410),
+                    __byte_perm(w.y, w.w, 0x7632));
+}
+__device__ __forceinline__ void fadd2(float2 &acc, float2 a) {
+  uint64_t d = (static_cast<uint64_t>(__float_as_uint(acc.y)) << 32) | __float_as_uint(acc.x);
+  const uint64_t x = (static_cast<uint64_t>(__float_as_uint(a.y)) << 32) | __float_as_uint(a.x);
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(d) : "l"(x));
+  acc.x = __uint_as_float(static_cast<uint32_t>(d));
+  acc.y = __uint_as_float(static_cast<uint32_t>(d >> 32));
+}
+
+// Eight channels of one token from their codes, packed as (0,4), (1,5),
+// (2,6), (3,7).
 template <bool BF16> __device__ __forceinline__ uint4 restore_row(uint32_t w, uint32_t scale, uint32_t low) {
-  uint32_t v[4]; // channels (0,4), (1,5), (2,6), (3,7)
+  uint32_t v[4];
   if constexpr (BF16) {
     const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162 *>(&scale);
     const __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162 *>(&low);
@@ -137,8 +154,7 @@ template <bool BF16> __device__ __forceinline__ uint4 restore_row(uint32_t w, ui
       v[i] = *reinterpret_cast<const uint32_t *>(&r);
     }
   }
-  return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
-                    __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+  return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 template <int D, bool BF16>
@@ -229,7 +245,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
       for (int c = 0; c < D / 8; ++c) {
         uint4 w = live ? src[c] : make_uint4(0, 0, 0, 0);
         w.x ^= g.flip, w.y ^= g.flip, w.z ^= g.flip, w.w ^= g.flip;
-        sts_v4(dst + (c / 8) * kAtom + (((c & 7) ^ (row & 7)) << 4), w);
+        sts_v4(dst + (c / 8) * kAtom + (((c & 7) ^ (row & 7)) << 4), interleave(w));
       }
       fence_async_smem();
       mbar_arrive(q_full);
@@ -251,21 +267,32 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         // one those at or past `from` or below `first`.
         const int to = pos - key0, from = g.window > 0 ? to - g.window : -1, first = g.sinks - key0;
         auto seen = [&](int c) { return c <= to && (c > from || c < first); };
-        float top = -INFINITY;
+        // Walks the row's 128 scores in chunks of 32, the next chunk on its
+        // way out of TMEM meanwhile.
+        auto walk = [&](auto body) {
+          uint32_t s[2][32];
+          tmem_ld32(t_s, s[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t s[32];
-          tmem_ld32(t_s + 32 * c, s);
-          tmem_ld_wait();
-          if (clear) {
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_wait();
+            if (c < 3)
+              tmem_ld32(t_s + 32 * (c + 1), s[(c + 1) & 1]);
+            body(c, s[c & 1]);
+          }
+        };
+        float top = -INFINITY;
+        if (clear) {
+          walk([&](int, const uint32_t (&s)[32]) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               top = fmaxf(top, __uint_as_float(s[e]));
-          } else {
+          });
+        } else {
+          walk([&](int c, const uint32_t (&s)[32]) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               top = fmaxf(top, seen(32 * c + e) ? __uint_as_float(s[e]) : -INFINITY);
-          }
+          });
         }
         const float up = fmaxf(m, top * g.scale_log2);
         if (__any_sync(~0u, up > m + 8.f)) {
@@ -286,30 +313,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
           }
         }
         const float minus = m == -INFINITY ? 0.f : -m;
-        float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t s[32], p[16];
-          tmem_ld32(t_s + 32 * c, s);
-          tmem_ld_wait();
+        float2 sum = make_float2(0.f, 0.f), sum2 = sum;
+        auto powers = [&](int c, const uint32_t (&s)[32], auto masked) {
+          uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             float2 x = make_float2(minus, minus);
             ffma2(x, make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
                   make_float2(g.scale_log2, g.scale_log2));
-            if (!clear) {
+            if constexpr (masked.value) {
               x.x = seen(32 * c + e) ? x.x : -INFINITY;
               x.y = seen(32 * c + e + 1) ? x.y : -INFINITY;
             }
             x.x = ex2_ftz(x.x);
             x.y = ex2_ftz(x.y);
-            sum.x += x.x;
-            sum.y += x.y;
+            fadd2(e & 2 ? sum2 : sum, x);
             p[e / 2] = kv4_pack<BF16>(x.x, x.y);
           }
+          // The columns of P lie within those of S that are read already.
           tmem_st16(t_s + 16 * c, p);
-        }
-        l += sum.x + sum.y;
+        };
+        if (clear)
+          walk([&](int c, const uint32_t (&s)[32]) { powers(c, s, std::false_type{}); });
+        else
+          walk([&](int c, const uint32_t (&s)[32]) { powers(c, s, std::true_type{}); });
+        l += (sum.x + sum2.x) + (sum.y + sum2.y);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(p_full + block);
@@ -331,44 +359,63 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               uint4 w;
-              w.x = kv4_pack<BF16>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
-              w.y = kv4_pack<BF16>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
-              w.z = kv4_pack<BF16>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
-              w.w = kv4_pack<BF16>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
+              w.x = kv4_pack<BF16>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 2]) * f);
+              w.y = kv4_pack<BF16>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 6]) * f);
+              w.z = kv4_pack<BF16>(__uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 3]) * f);
+              w.w = kv4_pack<BF16>(__uint_as_float(o[e + 5]) * f, __uint_as_float(o[e + 7]) * f);
               *reinterpret_cast<uint4 *>(dst + 32 * c + e) = w;
             }
         }
       }
     }
-  } else if (tiles > 0 && warp < 12) {
+  } else if (tiles > 0 && warp < 16) {
     // ----------------------------------------------------------- restoring
-    const int w = tid - 256;
+    const bool values = warp >= 12;
+    const int w = tid & 127;
     constexpr int kPer = 128 / G; // tokens a pass
     const int page = 1 << g.t.page_shift;
     const int tok0 = w / G, c = w % G; // token of the pass, group
-    uint4 kc[G], vc[G];
-    uint32_t kp[G], vp[G];
-    auto fetch = [&](int j) {
+    uint64_t *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
+    const uint32_t operand = sbase + (values ? L::kOffV : L::kOffK) + (c / 2) * kAtom;
+    const uint8_t *codes0 = g.pool + c * 16 + (values ? page * (D / 2) : 0);
+    const uint8_t *params0 = g.pool + page * D + c * 4 + (values ? page * (D / 8) : 0);
+    const long long block_bytes = static_cast<long long>(page) * (D + D / 4);
+    int ids[G]; // pages of the next tile's tokens, -1 past the length
+    uint4 codes[G];
+    uint32_t params[G];
+    auto find = [&](int j) {
       const int key0 = key_of_tile(j);
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         const int key = key0 + i * kPer + tok0;
-        kc[i] = vc[i] = make_uint4(0, 0, 0, 0);
-        kp[i] = vp[i] = 0; // past the length: zeros
-        if (key < seq.len) {
-          const long long p = kv4_page(g.t, b, key);
-          const int slot = key & (page - 1);
-          const uint8_t *blk = g.pool + (p * g.kv_heads + h) * static_cast<long long>(page * (D + D / 4));
-          const uint8_t *codes = blk + slot * (D / 2) + c * 16;
-          const uint8_t *params = blk + page * D + slot * (D / 8) + c * 4;
-          kc[i] = __ldg(reinterpret_cast<const uint4 *>(codes));
-          vc[i] = __ldg(reinterpret_cast<const uint4 *>(codes + page * (D / 2)));
-          kp[i] = __ldg(reinterpret_cast<const uint32_t *>(params));
-          vp[i] = __ldg(reinterpret_cast<const uint32_t *>(params + page * (D / 8)));
+        ids[i] = j < tiles && key < seq.len ? kv4_page(g.t, b, key) : -1;
+      }
+    };
+    auto fetch = [&](int j) {
+      const int key0 = key_of_tile(j);
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        codes[i] = make_uint4(0, 0, 0, 0);
+        params[i] = 0; // past the length: zeros
+        if (ids[i] >= 0) {
+          const long long at = (static_cast<long long>(ids[i]) * g.kv_heads + h) * block_bytes;
+          const int slot = (key0 + i * kPer + tok0) & (page - 1);
+          codes[i] = __ldg(reinterpret_cast<const uint4 *>(codes0 + at + slot * (D / 2)));
+          params[i] = __ldg(reinterpret_cast<const uint32_t *>(params0 + at + slot * (D / 8)));
         }
       }
     };
-    auto put = [&](uint32_t base, const uint4 (&codes)[G], const uint32_t (&params)[G]) {
+    find(0);
+    fetch(0);
+    find(1);
+    for (int j = 0; j < tiles; ++j) {
+      const int st = j & 1;
+      if (j >= 2) {
+        ok = mbar_wait(empty + st, (j / 2 - 1) & 1, abort);
+        ok = __all_sync(~0u, ok);
+        if (!ok)
+          break;
+      }
 #pragma unroll
       for (int i = 0; i < G; ++i) {
         const int tok = i * kPer + tok0;
@@ -378,37 +425,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         const bool turn = c >= 2;
         const uint32_t in[4] = {turn ? codes[i].z : codes[i].x, turn ? codes[i].w : codes[i].y,
                                 turn ? codes[i].x : codes[i].z, turn ? codes[i].y : codes[i].w};
-        const uint32_t row = base + (c / 2) * kAtom + tok * 128;
+        const uint32_t row = operand + st * L::kOperand + tok * 128;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int chunk = (c & 1) * 4 + (turn ? e ^ 2 : e);
           sts_v4(row + ((chunk ^ (tok & 7)) << 4), restore_row<BF16>(in[e], scale, low));
         }
       }
-    };
-    fetch(0);
-    for (int j = 0; j < tiles; ++j) {
-      const int st = j & 1;
-      if (j >= 2) {
-        ok = mbar_wait(k_empty + st, (j / 2 - 1) & 1, abort);
-        ok = __all_sync(~0u, ok);
-        if (!ok)
-          break;
-      }
-      put(sbase + L::kOffK + st * L::kOperand, kc, kp);
-      fence_async_smem();
-      mbar_arrive(k_full + st);
-      if (j >= 2) {
-        ok = mbar_wait(v_empty + st, (j / 2 - 1) & 1, abort);
-        ok = __all_sync(~0u, ok);
-        if (!ok)
-          break;
-      }
-      put(sbase + L::kOffV + st * L::kOperand, vc, vp);
-      fence_async_smem();
-      mbar_arrive(v_full + st);
-      if (j + 1 < tiles)
+      if (j + 1 < tiles) {
         fetch(j + 1);
+        find(j + 2);
+      }
+      fence_async_smem();
+      mbar_arrive(full + st);
     }
   } else if (tiles > 0 && lane == 0) {
     // ------------------------------------------------------------- issuing
