@@ -4,17 +4,18 @@
 // A CTA owns 256 query rows of one (sequence, key head): rows are (token,
 // head of the group) pairs, so the heads that share a key head share its
 // restored keys and values. It walks the 128-key tiles that its rows see:
-//  * four warps restore the tile's keys and four its values from the cache's
-//    pages (two codes a byte, scale * c + minimum rounded once to the cache's
+//  * seven warps restore the tile's keys and values from the cache's pages
+//    (two codes a byte, scale * c + minimum rounded once to the cache's
 //    16-bit type) into shared memory, as rows of a token, 128-byte swizzled;
-//    the next tile's codes are in registers and the page ids of the one after
-//    by then. Channels lie in the order 0 4 1 5 2 6 3 7 of every eight, as the
+//    the next tile's codes are in registers by then. Channels lie in the order 0 4 1 5 2 6 3 7 of every eight, as the
 //    codes' masks give them: queries are reordered alike, the output back;
 //  * one thread issues S = Q K^T for two blocks of 128 rows (K is K-major)
 //    and O += P V (V as it lies is the MN-major operand, P comes from TMEM);
 //  * four warps per block of rows, one row a thread, turn S into P in place:
 //    the fp32 score's columns become 16-bit probabilities in the first half
-//    of the same TMEM columns. The running maximum is only raised when a score
+//    of the same TMEM columns. A row's 128 scores come out of TMEM at once (a
+//    load's latency is several hundred cycles while products run) and stay in
+//    registers, which the restoring warps give up for that. The running maximum is only raised when a score
 //    passes it by more than 8 (in powers of two), so O in TMEM is rescaled
 //    rarely; while one block's rows are in the softmax, the other's products
 //    run.
@@ -30,7 +31,12 @@
 namespace pb2 {
 namespace {
 
-constexpr int kPromptThreads = 17 * 32; // 2 x 4 softmax warps, 2 x 4 restoring, 1 issuing
+constexpr int kPromptThreads = 16 * 32; // 2 x 4 softmax warps, 7 restoring, 1 issuing
+constexpr int kRestoreWarps = 7;
+// Registers a thread: launched with 128, of which the two warpgroups of
+// restoring and issuing warps keep 80 and the two of softmax warps get 176.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kOtherRegs = 80;
+static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "taken from the launch's own registers");
 constexpr int kTile = 128;
 constexpr int kBlockRows = 256;
 constexpr uint32_t kAtom = 128 * 128; // 128 rows of 128 bytes
@@ -93,16 +99,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
                : "r"(taddr)
                : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-               "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-               "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-               "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-               "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-               "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-               : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
                "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -116,6 +112,16 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ uint4 interleave(uint4 w) {
   return make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410),
                     __byte_perm(w.y, w.w, 0x7632));
+}
+// a * b + c and acc + a in pairs, each rounded once.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
 __device__ __forceinline__ void fadd2(float2 &acc, float2 a) {
   uint64_t d = (static_cast<uint64_t>(__float_as_uint(acc.y)) << 32) | __float_as_uint(acc.x);
@@ -174,8 +180,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
   if (tid == 0) {
     mbar_init(q_full, 256);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(k_full + i, 128);
-      mbar_init(v_full + i, 128);
+      mbar_init(k_full + i, kRestoreWarps);
+      mbar_init(v_full + i, kRestoreWarps);
       mbar_init(k_empty + i, 1);
       mbar_init(v_empty + i, 1);
       mbar_init(s_full + i, 1);
@@ -230,6 +236,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 
   if (tiles > 0 && warp < 8) {
     // ------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int block = warp >> 2;
     const int row = tid & 127; // within the block of 128
     const int r = block * 128 + row;
@@ -263,80 +270,81 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         const int key0 = key_of_tile(j);
         const bool clear = key0 + kTile - 1 <= pos_lo &&
                            (g.window <= 0 || key0 > pos_hi - g.window || key0 + kTile <= g.sinks);
-        // Key offsets that this row sees: [0, to) without a window, and with
-        // one those at or past `from` or below `first`.
-        const int to = pos - key0, from = g.window > 0 ? to - g.window : -1, first = g.sinks - key0;
-        auto seen = [&](int c) { return c <= to && (c > from || c < first); };
-        // Walks the row's 128 scores in chunks of 32, the next chunk on its
-        // way out of TMEM meanwhile.
-        auto walk = [&](auto body) {
-          uint32_t s[2][32];
-          tmem_ld32(t_s, s[0]);
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          tmem_ld32(t_s + 32 * c, s[c]);
+        tmem_ld_wait();
+        uint32_t none = 0; // chunks of 32 keys that no row of the warp sees
+        if (!clear) {
+          // Key offsets that this row sees: up to `to`, and with a window
+          // those past `from` or below `first`.
+          const int to = pos - key0, from = to - g.window, first = g.sinks - key0;
+          auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }; // bits 0 .. n - 1
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            tmem_ld_wait();
-            if (c < 3)
-              tmem_ld32(t_s + 32 * (c + 1), s[(c + 1) & 1]);
-            body(c, s[c & 1]);
+            uint32_t see = below(to + 1 - 32 * c);
+            if (g.window > 0)
+              see &= ~below(from + 1 - 32 * c) | below(first - 32 * c);
+            if (__all_sync(~0u, see == 0u)) {
+              none |= 1u << c;
+            } else if (!__all_sync(~0u, see == ~0u)) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                s[c][e] = see >> e & 1 ? s[c][e] : 0xFF800000u; // -inf
+            }
           }
-        };
-        float top = -INFINITY;
-        if (clear) {
-          walk([&](int, const uint32_t (&s)[32]) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              top = fmaxf(top, __uint_as_float(s[e]));
-          });
-        } else {
-          walk([&](int c, const uint32_t (&s)[32]) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              top = fmaxf(top, seen(32 * c + e) ? __uint_as_float(s[e]) : -INFINITY);
-          });
         }
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (!(none >> c & 1)) {
+            float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              tops[e / 2 % 4] = fmaxf(fmaxf(tops[e / 2 % 4], __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
+            top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+          }
         const float up = fmaxf(m, top * g.scale_log2);
         if (__any_sync(~0u, up > m + 8.f)) {
           const float f = up > m ? ex2_ftz(m - up) : 1.f;
           m = up;
           l *= f;
           if (j > 0) {
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(t_o + 32 * c, o);
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16]; // few at a time: the scores are in registers too
+              tmem_ld16(t_o + 16 * c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
+              for (int e = 0; e < 16; ++e)
                 o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st32(t_o + 32 * c, o);
+              tmem_st16(t_o + 16 * c, o);
             }
           }
         }
         const float minus = m == -INFINITY ? 0.f : -m;
         float2 sum = make_float2(0.f, 0.f), sum2 = sum;
-        auto powers = [&](int c, const uint32_t (&s)[32], auto masked) {
-          uint32_t p[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float2 x = make_float2(minus, minus);
-            ffma2(x, make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
-                  make_float2(g.scale_log2, g.scale_log2));
-            if constexpr (masked.value) {
-              x.x = seen(32 * c + e) ? x.x : -INFINITY;
-              x.y = seen(32 * c + e + 1) ? x.y : -INFINITY;
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
+          if (none >> c & 1) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              p[e] = 0;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float2 x = fma2(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])),
+                              make_float2(g.scale_log2, g.scale_log2), make_float2(minus, minus));
+              x.x = ex2_ftz(x.x);
+              x.y = ex2_ftz(x.y);
+              fadd2(e & 2 ? sum2 : sum, x);
+              p[e / 2] = kv4_pack<BF16>(x.x, x.y);
             }
-            x.x = ex2_ftz(x.x);
-            x.y = ex2_ftz(x.y);
-            fadd2(e & 2 ? sum2 : sum, x);
-            p[e / 2] = kv4_pack<BF16>(x.x, x.y);
           }
-          // The columns of P lie within those of S that are read already.
           tmem_st16(t_s + 16 * c, p);
-        };
-        if (clear)
-          walk([&](int c, const uint32_t (&s)[32]) { powers(c, s, std::false_type{}); });
-        else
-          walk([&](int c, const uint32_t (&s)[32]) { powers(c, s, std::true_type{}); });
+        }
         l += (sum.x + sum2.x) + (sum.y + sum2.y);
         tmem_st_wait();
         tc_fence_before();
@@ -368,132 +376,146 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         }
       }
     }
-  } else if (tiles > 0 && warp < 16) {
-    // ----------------------------------------------------------- restoring
-    const bool values = warp >= 12;
-    const int w = tid & 127;
-    constexpr int kPer = 128 / G; // tokens a pass
-    const int page = 1 << g.t.page_shift;
-    const int tok0 = w / G, c = w % G; // token of the pass, group
-    uint64_t *full = values ? v_full : k_full, *empty = values ? v_empty : k_empty;
-    const uint32_t operand = sbase + (values ? L::kOffV : L::kOffK) + (c / 2) * kAtom;
-    const uint8_t *codes0 = g.pool + c * 16 + (values ? page * (D / 2) : 0);
-    const uint8_t *params0 = g.pool + page * D + c * 4 + (values ? page * (D / 8) : 0);
-    const long long block_bytes = static_cast<long long>(page) * (D + D / 4);
-    int ids[G]; // pages of the next tile's tokens, -1 past the length
-    uint4 codes[G];
-    uint32_t params[G];
-    auto find = [&](int j) {
-      const int key0 = key_of_tile(j);
+  } else if (tiles > 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp < 8 + kRestoreWarps) {
+      // ----------------------------------------------------------- restoring
+      // A piece is 32 / G tokens of one operand: 16 bytes of codes a lane. Keys
+      // come first; the warps take them in turn.
+      constexpr int kTokens = 32 / G, kPieces = 4 * G; // of one operand
+      constexpr int kMine = (2 * kPieces + kRestoreWarps - 1) / kRestoreWarps;
+      const int w = warp - 8;
+      const int page = 1 << g.t.page_shift;
+      const int tok0 = lane / G, c = lane % G; // token of the piece, group
+      const long long block_bytes = static_cast<long long>(page) * (D + D / 4);
+      const uint8_t *mine = g.pool + h * block_bytes;
+      uint4 codes[kMine];
+      uint32_t params[kMine];
+      auto fetch = [&](int j) {
+        const int key0 = key_of_tile(j);
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
-        const int key = key0 + i * kPer + tok0;
-        ids[i] = j < tiles && key < seq.len ? kv4_page(g.t, b, key) : -1;
-      }
-    };
-    auto fetch = [&](int j) {
-      const int key0 = key_of_tile(j);
-#pragma unroll
-      for (int i = 0; i < G; ++i) {
-        codes[i] = make_uint4(0, 0, 0, 0);
-        params[i] = 0; // past the length: zeros
-        if (ids[i] >= 0) {
-          const long long at = (static_cast<long long>(ids[i]) * g.kv_heads + h) * block_bytes;
-          const int slot = (key0 + i * kPer + tok0) & (page - 1);
-          codes[i] = __ldg(reinterpret_cast<const uint4 *>(codes0 + at + slot * (D / 2)));
-          params[i] = __ldg(reinterpret_cast<const uint32_t *>(params0 + at + slot * (D / 8)));
+        for (int i = 0; i < kMine; ++i) {
+          const int piece = w + i * kRestoreWarps;
+          const int values = piece >= kPieces;
+          const int key = key0 + (piece - values * kPieces) * kTokens + tok0;
+          codes[i] = make_uint4(0, 0, 0, 0);
+          params[i] = 0; // past the length: zeros
+          if (piece < 2 * kPieces && key < seq.len) {
+            const uint8_t *blk = mine + kv4_page(g.t, b, key) * (block_bytes * g.kv_heads);
+            const int slot = (key & (page - 1)) + values * page;
+            codes[i] = __ldg(reinterpret_cast<const uint4 *>(blk + slot * (D / 2) + c * 16));
+            params[i] = __ldg(reinterpret_cast<const uint32_t *>(blk + page * D + slot * (D / 8) + c * 4));
+          }
         }
-      }
-    };
-    find(0);
-    fetch(0);
-    find(1);
-    for (int j = 0; j < tiles; ++j) {
-      const int st = j & 1;
-      if (j >= 2) {
-        ok = mbar_wait(empty + st, (j / 2 - 1) & 1, abort);
-        ok = __all_sync(~0u, ok);
-        if (!ok)
-          break;
-      }
-#pragma unroll
-      for (int i = 0; i < G; ++i) {
-        const int tok = i * kPer + tok0;
+      };
+      auto put = [&](int i, uint32_t operand) {
+        const int piece = w + i * kRestoreWarps;
+        const int tok = (piece >= kPieces ? piece - kPieces : piece) * kTokens + tok0;
         const uint32_t scale = __byte_perm(params[i], 0, 0x1010), low = __byte_perm(params[i], 0, 0x3232);
         // Lanes of the upper two groups write their chunks in another order,
         // so that the eight lanes of a phase meet eight bank columns.
         const bool turn = c >= 2;
         const uint32_t in[4] = {turn ? codes[i].z : codes[i].x, turn ? codes[i].w : codes[i].y,
                                 turn ? codes[i].x : codes[i].z, turn ? codes[i].y : codes[i].w};
-        const uint32_t row = operand + st * L::kOperand + tok * 128;
+        const uint32_t row = operand + (c / 2) * kAtom + tok * 128;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int chunk = (c & 1) * 4 + (turn ? e ^ 2 : e);
           sts_v4(row + ((chunk ^ (tok & 7)) << 4), restore_row<BF16>(in[e], scale, low));
         }
-      }
-      if (j + 1 < tiles) {
-        fetch(j + 1);
-        find(j + 2);
-      }
-      fence_async_smem();
-      mbar_arrive(full + st);
-    }
-  } else if (tiles > 0 && lane == 0) {
-    // ------------------------------------------------------------- issuing
-    constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
-    constexpr uint32_t idesc_s = idesc_f16_f32(128, 128) | kType;
-    constexpr uint32_t idesc_o = idesc_f16_f32(128, D) | kType | (1u << 16); // B is MN-major
-    auto scores = [&](int block, int st) {
+      };
+      fetch(0);
+      for (int j = 0; j < tiles; ++j) {
+        const int st = j & 1;
+        if (j >= 2) {
+          ok = mbar_wait(k_empty + st, (j / 2 - 1) & 1, abort);
+          ok = __all_sync(~0u, ok);
+          if (!ok)
+            break;
+        }
+        // Pieces below kPieces are keys: all of a warp's first ones, some of
+        // the next.
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = (k / 4) * kAtom + (k & 3) * 32;
-        umma_f16(tmem + block * 128, sdesc_k_sw128(sbase + L::kOffQ + block * L::kOperand + off),
-                 sdesc_k_sw128(sbase + L::kOffK + st * L::kOperand + off), idesc_s, k != 0);
-      }
-      umma_commit(s_full + block);
-    };
-    auto values = [&](int block, int st, int j) {
+        for (int i = 0; i < kMine; ++i)
+          if (w + i * kRestoreWarps < kPieces)
+            put(i, sbase + L::kOffK + st * L::kOperand);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(k_full + st);
+        if (j >= 2) {
+          ok = mbar_wait(v_empty + st, (j / 2 - 1) & 1, abort);
+          ok = __all_sync(~0u, ok);
+          if (!ok)
+            break;
+        }
 #pragma unroll
-      for (int k = 0; k < kTile / 16; ++k)
-        umma_ts(tmem + 256 + block * 128, tmem + block * 128 + k * 8,
-                sdesc_mn_sw128(sbase + L::kOffV + st * L::kOperand + k * 2048), idesc_o, j != 0 || k != 0);
-    };
-    ok = mbar_wait(q_full, 0, abort) && mbar_wait(k_full, 0, abort);
-    if (ok) {
-      tc_fence_after();
-      scores(0, 0);
-      if (two)
-        scores(1, 0);
-      umma_commit(k_empty);
-    }
-    for (int j = 0; ok && j < tiles; ++j) {
-      const int st = j & 1, next = st ^ 1;
-      const bool more = j + 1 < tiles;
-      ok = mbar_wait(v_full + st, (j / 2) & 1, abort) && (!more || mbar_wait(k_full + next, ((j + 1) / 2) & 1, abort));
-      for (int block = 0; ok && block < (two ? 2 : 1); ++block) {
-        ok = mbar_wait(p_full + block, j & 1, abort);
-        if (!ok)
-          break;
-        tc_fence_after();
-        values(block, st, j);
-        if (more)
-          scores(block, next);
-        else
-          umma_commit(o_full + block);
+        for (int i = 0; i < kMine; ++i)
+          if (w + i * kRestoreWarps >= kPieces && w + i * kRestoreWarps < 2 * kPieces)
+            put(i, sbase + L::kOffV + st * L::kOperand);
+        if (j + 1 < tiles)
+          fetch(j + 1);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(v_full + st);
       }
+    } else if (lane == 0) {
+      // ------------------------------------------------------------- issuing
+      constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
+      constexpr uint32_t idesc_s = idesc_f16_f32(128, 128) | kType;
+      constexpr uint32_t idesc_o = idesc_f16_f32(128, D) | kType | (1u << 16); // B is MN-major
+      auto scores = [&](int block, int st) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k / 4) * kAtom + (k & 3) * 32;
+          umma_f16(tmem + block * 128, sdesc_k_sw128(sbase + L::kOffQ + block * L::kOperand + off),
+                   sdesc_k_sw128(sbase + L::kOffK + st * L::kOperand + off), idesc_s, k != 0);
+        }
+        umma_commit(s_full + block);
+      };
+      auto values = [&](int block, int st, int j) {
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          umma_ts(tmem + 256 + block * 128, tmem + block * 128 + k * 8,
+                  sdesc_mn_sw128(sbase + L::kOffV + st * L::kOperand + k * 2048), idesc_o, j != 0 || k != 0);
+      };
+      ok = mbar_wait(q_full, 0, abort) && mbar_wait(k_full, 0, abort);
       if (ok) {
-        umma_commit(v_empty + st);
-        if (more)
-          umma_commit(k_empty + next);
+        tc_fence_after();
+        scores(0, 0);
+        if (two)
+          scores(1, 0);
+        umma_commit(k_empty);
       }
-    }
-    if (!ok) {
-      // Everything issued ends before the memory goes away.
-      *abort = 1;
-      umma_commit(drain);
-      const long long t0 = clock64();
-      while (!mbar_try_wait(drain, 0) && clock64() - t0 < kWaitBudgetCycles) {
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int st = j & 1, next = st ^ 1;
+        const bool more = j + 1 < tiles;
+        ok = mbar_wait(v_full + st, (j / 2) & 1, abort) && (!more || mbar_wait(k_full + next, ((j + 1) / 2) & 1, abort));
+        for (int block = 0; ok && block < (two ? 2 : 1); ++block) {
+          ok = mbar_wait(p_full + block, j & 1, abort);
+          if (!ok)
+            break;
+          tc_fence_after();
+          values(block, st, j);
+          if (more)
+            scores(block, next);
+          else
+            umma_commit(o_full + block);
+        }
+        if (ok) {
+          umma_commit(v_empty + st);
+          if (more)
+            umma_commit(k_empty + next);
+        }
+      }
+      if (!ok) {
+        // Everything issued ends before the memory goes away.
+        *abort = 1;
+        umma_commit(drain);
+        const long long t0 = clock64();
+        while (!mbar_try_wait(drain, 0) && clock64() - t0 < kWaitBudgetCycles) {
+        }
       }
     }
   }
@@ -515,6 +537,13 @@ template <int D, bool BF16> cudaError_t launch_prompt(const PromptArgs &g, cudaS
                                        static_cast<int>(PromptLayout<D>::kBytes));
   if (e != cudaSuccess)
     return e;
+  // The softmax warps wait for registers that the launch must have brought.
+  cudaFuncAttributes attr;
+  e = cudaFuncGetAttributes(&attr, kernel);
+  if (e != cudaSuccess)
+    return e;
+  if (attr.numRegs < kLaunchRegs)
+    return cudaErrorInvalidConfiguration;
   const unsigned grid = static_cast<unsigned>(g.row_blocks) * g.t.batch * g.kv_heads;
   return launch_pdl(kernel, grid, kPromptThreads, PromptLayout<D>::kBytes, stream, g);
 }
@@ -533,7 +562,8 @@ cudaError_t kv4_attend_prompt(const Kv4Cache &c, const Kv4Tokens &t, const Kv4At
   g.group = a.heads / c.kv_heads;
   g.window = a.window;
   g.sinks = a.sinks;
-  g.scale_log2 = fabsf(a.scale) * kLog2e;
+  // Not 0: hidden scores are -inf before the scale is applied.
+  g.scale_log2 = std::max(fabsf(a.scale) * kLog2e, 1e-30f);
   g.flip = a.scale < 0.f ? 0x80008000u : 0u;
   const long long blocks = (static_cast<long long>(t.max_new) * g.group + kBlockRows - 1) / kBlockRows;
   // Block indices are divided in 31 bits.
