@@ -113,6 +113,11 @@ __device__ __forceinline__ uint4 interleave(uint4 w) {
   return make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410),
                     __byte_perm(w.y, w.w, 0x7632));
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // a * b + c and acc + a in pairs, each rounded once.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -242,17 +247,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     const int r = block * 128 + row;
     const bool live = r < rows;
     const uint32_t i = g.group_div.div(row0 + r);
-    const int head = h * g.group + static_cast<int>(row0 + r - i * g.group);
     const int pos = live ? past + static_cast<int>(i) : -1;
+    // A warp moves its 32 rows, neighbouring lanes along a row: the heads of a
+    // token's group lie side by side.
+    const uint32_t own_rows = sbase + L::kOffQ + block * L::kOperand + (warp & 3) * 32 * 128;
+    auto chunk_at = [&](int rr, int c) { return own_rows + (c / 8) * kAtom + rr * 128 + (((c & 7) ^ (rr & 7)) << 4); };
+    const int warp_row = block * 128 + (warp & 3) * 32;
+    auto offset_of = [&](int rr, long long stride) { // of a row's first element
+      const uint32_t n = row0 + warp_row + rr, i = g.group_div.div(n);
+      return (seq.first + static_cast<long long>(i)) * stride + (h * g.group + static_cast<int>(n - i * g.group)) * D;
+    };
     {
-      const uint4 *src =
-          reinterpret_cast<const uint4 *>(g.q + (seq.first + static_cast<long long>(i)) * g.q_stride + head * D);
-      const uint32_t dst = sbase + L::kOffQ + block * L::kOperand + row * 128;
+      uint4 w[D / 8]; // all loads first
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 w = live ? src[c] : make_uint4(0, 0, 0, 0);
-        w.x ^= g.flip, w.y ^= g.flip, w.z ^= g.flip, w.w ^= g.flip;
-        sts_v4(dst + (c / 8) * kAtom + (((c & 7) ^ (row & 7)) << 4), interleave(w));
+      for (int it = 0; it < D / 8; ++it) {
+        const int rr = (it * 32 + lane) / (D / 8), c = lane % (D / 8);
+        w[it] = make_uint4(0, 0, 0, 0);
+        if (warp_row + rr < rows)
+          w[it] = __ldg(reinterpret_cast<const uint4 *>(g.q + offset_of(rr, g.q_stride)) + c);
+      }
+#pragma unroll
+      for (int it = 0; it < D / 8; ++it) {
+        const int rr = (it * 32 + lane) / (D / 8), c = lane % (D / 8);
+        w[it].x ^= g.flip, w[it].y ^= g.flip, w[it].z ^= g.flip, w[it].w ^= g.flip;
+        sts_v4(chunk_at(rr, c), interleave(w[it]));
       }
       fence_async_smem();
       mbar_arrive(q_full);
@@ -302,8 +320,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             float tops[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int e = 0; e < 32; e += 2)
-              tops[e / 2 % 4] = fmaxf(fmaxf(tops[e / 2 % 4], __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
-            top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+              tops[e / 2 % 4] = max3(tops[e / 2 % 4], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+            top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]);
           }
         const float up = fmaxf(m, top * g.scale_log2);
         if (__any_sync(~0u, up > m + 8.f)) {
@@ -333,14 +351,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             for (int e = 0; e < 16; ++e)
               p[e] = 0;
           } else {
+            // Three stages on pairs of scores (scale, power, sum and round),
+            // a few pairs apart: the special function unit takes eight cycles
+            // a warp for each power, and the rest fits in between only if
+            // it does not wait for the same pair.
+            constexpr int kApart = 3;
+            float2 x[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float2 x = fma2(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])),
-                              make_float2(g.scale_log2, g.scale_log2), make_float2(minus, minus));
-              x.x = ex2_ftz(x.x);
-              x.y = ex2_ftz(x.y);
-              fadd2(e & 2 ? sum2 : sum, x);
-              p[e / 2] = kv4_pack<BF16>(x.x, x.y);
+            for (int i = 0; i < 16 + 2 * kApart; ++i) {
+              if (i < 16)
+                x[i] = fma2(make_float2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])),
+                            make_float2(g.scale_log2, g.scale_log2), make_float2(minus, minus));
+              if (i >= kApart && i < 16 + kApart) {
+                x[i - kApart].x = ex2_ftz(x[i - kApart].x);
+                x[i - kApart].y = ex2_ftz(x[i - kApart].y);
+              }
+              if (i >= 2 * kApart) {
+                const int k = i - 2 * kApart;
+                fadd2(k & 1 ? sum2 : sum, x[k]);
+                p[k] = kv4_pack<BF16>(x[k].x, x[k].y);
+              }
             }
           }
           tmem_st16(t_s + 16 * c, p);
@@ -357,22 +387,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
       if (ok) {
         tc_fence_after();
         const float f = l > 0.f ? __fdividef(1.f, l) : l; // nothing seen: 0; NaN stays NaN
-        uint16_t *dst = g.out + ((seq.first + static_cast<long long>(i)) * g.heads + head) * D;
+        // Through the rows' place of the queries, which all products have
+        // read by now.
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(t_o + 32 * c, o);
           tmem_ld_wait();
-          if (live)
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint4 w;
-              w.x = kv4_pack<BF16>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 2]) * f);
-              w.y = kv4_pack<BF16>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 6]) * f);
-              w.z = kv4_pack<BF16>(__uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 3]) * f);
-              w.w = kv4_pack<BF16>(__uint_as_float(o[e + 5]) * f, __uint_as_float(o[e + 7]) * f);
-              *reinterpret_cast<uint4 *>(dst + 32 * c + e) = w;
-            }
+          for (int e = 0; e < 32; e += 8) {
+            uint4 w;
+            w.x = kv4_pack<BF16>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 2]) * f);
+            w.y = kv4_pack<BF16>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 6]) * f);
+            w.z = kv4_pack<BF16>(__uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 3]) * f);
+            w.w = kv4_pack<BF16>(__uint_as_float(o[e + 5]) * f, __uint_as_float(o[e + 7]) * f);
+            sts_v4(chunk_at(lane, 4 * c + e / 8), w);
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int it = 0; it < D / 8; ++it) {
+          const int rr = (it * 32 + lane) / (D / 8), c = lane % (D / 8);
+          if (warp_row + rr < rows)
+            reinterpret_cast<uint4 *>(g.out + offset_of(rr, static_cast<long long>(g.heads) * D))[c] =
+                lds_v4(chunk_at(rr, c));
         }
       }
     }
@@ -389,29 +427,43 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
       const int tok0 = lane / G, c = lane % G; // token of the piece, group
       const long long block_bytes = static_cast<long long>(page) * (D + D / 4);
       const uint8_t *mine = g.pool + h * block_bytes;
+      const long long page_stride = block_bytes * g.kv_heads;
+      const int *row = g.t.table + static_cast<long long>(b) * g.t.width;
       uint4 codes[kMine];
       uint32_t params[kMine];
-      auto fetch = [&](int j) {
-        const int key0 = key_of_tile(j);
+      int ids[kMine];     // page of the piece's tokens in the tile to fetch next
+      uint32_t place[kMine]; // of the piece's codes in the block
+      bool bad = false;
+      auto exists = [&](int i) { return w + i * kRestoreWarps < 2 * kPieces; };
+      auto is_value = [&](int i) { return w + i * kRestoreWarps >= kPieces; };
+      auto token_of = [&](int i) { return (w + i * kRestoreWarps - is_value(i) * kPieces) * kTokens + tok0; };
+      // A tile starts on a page's start, so a piece's slots are the same in
+      // every tile.
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int piece = w + i * kRestoreWarps;
-          const int values = piece >= kPieces;
-          const int key = key0 + (piece - values * kPieces) * kTokens + tok0;
-          codes[i] = make_uint4(0, 0, 0, 0);
-          params[i] = 0; // past the length: zeros
-          if (piece < 2 * kPieces && key < seq.len) {
-            const uint8_t *blk = mine + kv4_page(g.t, b, key) * (block_bytes * g.kv_heads);
-            const int slot = (key & (page - 1)) + values * page;
-            codes[i] = __ldg(reinterpret_cast<const uint4 *>(blk + slot * (D / 2) + c * 16));
-            params[i] = __ldg(reinterpret_cast<const uint32_t *>(blk + page * D + slot * (D / 8) + c * 4));
-          }
+      for (int i = 0; i < kMine; ++i)
+        place[i] = ((token_of(i) & (page - 1)) + is_value(i) * page) * (D / 2) + c * 16;
+      auto find = [&](int i, int j) {
+        const int key = key_of_tile(j) + token_of(i);
+        ids[i] = exists(i) && j < tiles && key < seq.len ? __ldg(row + (key >> g.t.page_shift)) : 0;
+      };
+      // Loads the piece of tile j, whose page id is there, and the page id
+      // of the next.
+      auto fetch = [&](int i, int j) {
+        if (exists(i) && j < tiles) {
+          bad = bad || static_cast<unsigned>(ids[i]) >= static_cast<unsigned>(g.t.pages);
+          const uint8_t *blk =
+              mine + min(static_cast<unsigned>(ids[i]), static_cast<unsigned>(g.t.pages - 1)) * page_stride;
+          codes[i] = __ldg(reinterpret_cast<const uint4 *>(blk + place[i]));
+          // D / 8 bytes of groups to D / 2 of codes.
+          params[i] = __ldg(reinterpret_cast<const uint32_t *>(blk + page * D + place[i] / 4));
+          find(i, j + 1);
         }
       };
-      auto put = [&](int i, uint32_t operand) {
-        const int piece = w + i * kRestoreWarps;
-        const int tok = (piece >= kPieces ? piece - kPieces : piece) * kTokens + tok0;
-        const uint32_t scale = __byte_perm(params[i], 0, 0x1010), low = __byte_perm(params[i], 0, 0x3232);
+      auto put = [&](int i, int j, uint32_t operand) {
+        const int tok = token_of(i);
+        // Past the length: zeros.
+        const uint32_t group = key_of_tile(j) + tok < seq.len ? params[i] : 0u;
+        const uint32_t scale = __byte_perm(group, 0, 0x1010), low = __byte_perm(group, 0, 0x3232);
         // Lanes of the upper two groups write their chunks in another order,
         // so that the eight lanes of a phase meet eight bank columns.
         const bool turn = c >= 2;
@@ -424,42 +476,42 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
           sts_v4(row + ((chunk ^ (tok & 7)) << 4), restore_row<BF16>(in[e], scale, low));
         }
       };
-      fetch(0);
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        find(i, 0);
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        fetch(i, 0);
       for (int j = 0; j < tiles; ++j) {
         const int st = j & 1;
-        if (j >= 2) {
-          ok = mbar_wait(k_empty + st, (j / 2 - 1) & 1, abort);
-          ok = __all_sync(~0u, ok);
-          if (!ok)
-            break;
-        }
-        // Pieces below kPieces are keys: all of a warp's first ones, some of
-        // the next.
 #pragma unroll
-        for (int i = 0; i < kMine; ++i)
-          if (w + i * kRestoreWarps < kPieces)
-            put(i, sbase + L::kOffK + st * L::kOperand);
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(k_full + st);
-        if (j >= 2) {
-          ok = mbar_wait(v_empty + st, (j / 2 - 1) & 1, abort);
-          ok = __all_sync(~0u, ok);
-          if (!ok)
-            break;
-        }
+        for (int values = 0; values < 2; ++values) {
+          if (j >= 2) {
+            ok = mbar_wait((values ? v_empty : k_empty) + st, (j / 2 - 1) & 1, abort);
+            ok = __all_sync(~0u, ok);
+            if (!ok)
+              break;
+          }
+          const uint32_t operand = sbase + (values ? L::kOffV : L::kOffK) + st * L::kOperand;
 #pragma unroll
-        for (int i = 0; i < kMine; ++i)
-          if (w + i * kRestoreWarps >= kPieces && w + i * kRestoreWarps < 2 * kPieces)
-            put(i, sbase + L::kOffV + st * L::kOperand);
-        if (j + 1 < tiles)
-          fetch(j + 1);
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(v_full + st);
+          for (int i = 0; i < kMine; ++i)
+            if (is_value(i) == values && exists(i))
+              put(i, j, operand);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive((values ? v_full : k_full) + st);
+          // On its way while the other operand is restored.
+#pragma unroll
+          for (int i = 0; i < kMine; ++i)
+            if (is_value(i) == values)
+              fetch(i, j + 1);
+        }
+        if (!ok)
+          break;
       }
+      if (bad)
+        kv4_fault(g.t, kErrPage);
     } else if (lane == 0) {
       // ------------------------------------------------------------- issuing
       constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
