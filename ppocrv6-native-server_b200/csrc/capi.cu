@@ -104,10 +104,10 @@ const char *kv4_arguments(const PpocrKv4Cache *cache, const int *table, int widt
   t.err = device_error_word();
   return nullptr;
 }
-// New tokens of one sequence, in 8-channel chunks of all key heads, are
-// counted in 32 bits.
+// New tokens of one sequence, in 8-channel chunks of all keys and values, are
+// counted in 31 bits.
 const char *kv4_row_arguments(const PpocrKv4Cache *cache, int max_new) {
-  return static_cast<long long>(max_new) * cache->kv_heads * (cache->head_dim / 8) >= (1ll << 31)
+  return static_cast<long long>(max_new) * cache->kv_heads * (cache->head_dim / 4) >= (1ll << 31) - (1 << 12)
              ? "max_new * kv_heads * head_dim is too large"
              : nullptr;
 }

@@ -1,17 +1,25 @@
 // Writing keys and values into the 4-bit cache, and reading them back.
 //
-// Both kernels move bytes: 4 per value come in (K and V, 16 bits each) and
-// 1.25 go out, or the other way round. A thread owns eight channels of one
-// (token, head) of K and of V: one 16-byte and one 4-byte access each, four
-// neighbouring lanes making a group of 32 channels, so the group's minimum
-// and maximum take two shuffles. Blocks are laid out over (new tokens of a
-// sequence) x (sequence): ragged batches leave blocks that only exit.
+// Both kernels move bytes: 4 per key-value pair of channels come in (16 bits
+// each) and 1.25 go out, or the other way round; next to that the append
+// kernel is close to being bound by its instructions (about nine a value).
+//  * append: a thread owns a group of 32 channels: four 16-byte loads, packed
+//    16-bit minimum and maximum, one division by 15 and one reciprocal per
+//    group, a 16-byte store of codes and a 4-byte one of (scale, minimum).
+//    Values that are not finite or beyond the limit are looked for in the bit
+//    patterns and put right on a path of their own.
+//  * read: a thread owns eight channels of a key and of its value, so that
+//    its 16-byte stores and its neighbours' are whole lines.
+// A thread takes several such items, all loads before the first use. Blocks
+// are laid out over (items of a sequence) x (sequence): ragged batches leave
+// blocks that only exit.
 #include "kv4.cuh"
 
 namespace pb2 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kAppendItems = 2, kReadItems = 2;
 
 struct CacheArgs {
   Kv4Tokens t;
@@ -20,28 +28,29 @@ struct CacheArgs {
   uint16_t *ko, *vo;     // read: destination rows
   long long k_stride, v_stride;
   int kv_heads;
-  FastDiv heads_div;
+  FastDiv token_div; // by the items of one token
 };
 
-// Where this thread's eight channels sit.
+// Where an item sits: `per` items to a head; with BOTH, all of a token's key
+// items come before its value items.
 struct Spot {
-  bool live;          // a token of this sequence
-  bool held;          // with a position in the cache
-  long long row;      // packed row
-  int head, chunk;    // eight-channel chunk of the head
-  uint8_t *block;     // (page, head) block
-  int slot;           // token within the page
+  bool live;      // of a token of this sequence
+  bool held;      // with a position in the cache
+  bool value;     // of the values, not the keys
+  int head, part; // part of the head
+  long long row;  // packed row
+  uint8_t *block; // (page, head) block
+  int slot;       // token within the page
 };
-template <int D> __device__ __forceinline__ Spot spot_of(const CacheArgs &g) {
-  constexpr int kChunks = D / 8;
+template <int D, bool BOTH>
+__device__ __forceinline__ Spot spot_of(const CacheArgs &g, const Kv4Seq &q, uint32_t item, int per) {
   Spot s;
-  const int b = blockIdx.y;
-  const Kv4Seq q = kv4_seq(g.t, b);
-  const uint32_t idx = blockIdx.x * kThreads + threadIdx.x;
-  s.chunk = idx % kChunks;
-  const uint32_t rest = idx / kChunks;
-  const uint32_t tok = g.heads_div.div(rest);
-  s.head = rest - tok * g.kv_heads;
+  const uint32_t tok = g.token_div.div(item);
+  const int in = item - tok * ((BOTH ? 2 : 1) * g.kv_heads * per);
+  s.value = BOTH && in >= g.kv_heads * per;
+  const int at = in - (s.value ? g.kv_heads * per : 0);
+  s.head = at / per; // a power of two
+  s.part = at % per;
   s.live = tok < static_cast<uint32_t>(q.n);
   const int pos = q.len - q.n + static_cast<int>(tok);
   s.held = s.live && pos >= 0;
@@ -49,116 +58,192 @@ template <int D> __device__ __forceinline__ Spot spot_of(const CacheArgs &g) {
   s.block = nullptr;
   s.slot = 0;
   if (s.held) {
-    const long long page = kv4_page(g.t, b, pos);
+    const long long page = kv4_page(g.t, blockIdx.y, pos);
     s.slot = pos & ((1 << g.t.page_shift) - 1);
     s.block = g.pool + (page * g.kv_heads + s.head) * static_cast<long long>((D + D / 4) << g.t.page_shift);
   }
   return s;
 }
 
-// Quantises eight channels (with the three lanes that hold the rest of the
-// group): returns the packed codes and the group's (scale, minimum).
-template <bool BF16> __device__ __forceinline__ uint32_t quantise8(uint4 w, uint32_t &params) {
-  const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-  constexpr float kMost = BF16 ? 8.507059173023462e37f : 65000.f; // 2^126
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = kv4_lo<BF16>(in[i]);
-    x[2 * i + 1] = kv4_hi<BF16>(in[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    x[i] = x[i] == x[i] ? fminf(fmaxf(x[i], -kMost), kMost) : 0.f;
-  float lo = x[0], hi = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-  }
-#pragma unroll
-  for (int o = 1; o < 4; o *= 2) {
-    lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
-  }
-  params = kv4_pack<BF16>(__fdiv_rn(__fsub_rn(hi, kv4_lo<BF16>(kv4_pack<BF16>(lo, lo))), 15.f), lo);
-  const float scale = kv4_lo<BF16>(params);
-  lo = kv4_hi<BF16>(params);
-  const float inv = scale > 1e-30f ? __fdiv_rn(1.f, scale) : 0.f;
-  uint32_t codes = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], lo), inv), 0.f), 15.f);
-    // Adding 1.5 * 2^23 rounds to the nearest whole number (ties to even)
-    // and leaves it in the low bits.
-    codes |= (__float_as_uint(__fadd_rn(c, 12582912.f)) & 15u) << (4 * i);
-  }
-  return codes;
+template <bool BF16> struct Packed;
+template <> struct Packed<false> {
+  using type = __half2;
+  static constexpr float kMost = 65000.f;
+  static constexpr uint32_t kMostBits = 0x7BEFu; // the largest value not above it
+};
+template <> struct Packed<true> {
+  using type = __nv_bfloat162;
+  static constexpr float kMost = 8.507059173023462e37f; // 2^126
+  static constexpr uint32_t kMostBits = 0x7E80u;
+};
+template <bool BF16> __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  using T = typename Packed<BF16>::type;
+  const T r = __hmin2(*reinterpret_cast<const T *>(&a), *reinterpret_cast<const T *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <bool BF16> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  using T = typename Packed<BF16>::type;
+  const T r = __hmax2(*reinterpret_cast<const T *>(&a), *reinterpret_cast<const T *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
-template <int D, bool BF16> __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ CacheArgs g) {
-  pdl_begin();
-  const Spot s = spot_of<D>(g);
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  if (s.held) {
-    const long long e = s.head * D + s.chunk * 8;
-    k = *reinterpret_cast<const uint4 *>(g.k + s.row * g.k_stride + e);
-    v = *reinterpret_cast<const uint4 *>(g.v + s.row * g.v_stride + e);
+// Quantises a group of 32 channels (16 words): its codes and its (scale,
+// minimum). Every step is rounded as the definition has it: the difference,
+// the product, then to the nearest whole number.
+template <bool BF16> __device__ __forceinline__ uint4 quantise(uint4 (&in)[4], uint32_t &params) {
+  uint32_t *w = reinterpret_cast<uint32_t *>(in);
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    most = __vmaxu2(most, w[i] & 0x7FFF7FFFu);
+  if ((most & 0xFFFFu) > Packed<BF16>::kMostBits || (most >> 16) > Packed<BF16>::kMostBits) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float a = kv4_lo<BF16>(w[i]), b = kv4_hi<BF16>(w[i]);
+      a = a == a ? fminf(fmaxf(a, -Packed<BF16>::kMost), Packed<BF16>::kMost) : 0.f;
+      b = b == b ? fminf(fmaxf(b, -Packed<BF16>::kMost), Packed<BF16>::kMost) : 0.f;
+      w[i] = kv4_pack<BF16>(a, b);
+    }
   }
-  uint32_t kp, vp;
-  const uint32_t kc = quantise8<BF16>(k, kp), vc = quantise8<BF16>(v, vp);
-  if (!s.held)
-    return;
+  uint32_t mn = w[0], mx = w[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) {
+    mn = min2<BF16>(mn, w[i]);
+    mx = max2<BF16>(mx, w[i]);
+  }
+  const float lo = fminf(kv4_lo<BF16>(mn), kv4_hi<BF16>(mn)), hi = fmaxf(kv4_lo<BF16>(mx), kv4_hi<BF16>(mx));
+  params = kv4_pack<BF16>(__fdiv_rn(__fsub_rn(hi, lo), 15.f), lo);
+  const float scale = kv4_lo<BF16>(params);
+  const float inv = scale > 1e-30f ? __frcp_rn(scale) : 0.f;
+  uint32_t codes[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    // Adding 1.5 * 2^23 rounds to the nearest whole number (ties to even) and
+    // leaves it in the low bits; the constant's own bits are taken off the
+    // eight at once.
+    uint32_t sum = 0;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+      const uint32_t x = w[4 * c + i];
+      float2 q = mul2(add2(make_float2(kv4_lo<BF16>(x), kv4_hi<BF16>(x)), make_float2(-lo, -lo)), make_float2(inv, inv));
+      // Never below 0; above 15 where a tiny scale was rounded down.
+      q.x = fminf(q.x, 15.f);
+      q.y = fminf(q.y, 15.f);
+      q = add2(q, make_float2(12582912.f, 12582912.f));
+      sum = (sum << 4) + __float_as_uint(q.y);
+      sum = (sum << 4) + __float_as_uint(q.x);
+    }
+    codes[c] = sum - 0x4B400000u * 0x11111111u;
+  }
+  return make_uint4(codes[0], codes[1], codes[2], codes[3]);
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ CacheArgs g) {
+  pdl_begin();
+  const Kv4Seq q = kv4_seq(g.t, blockIdx.y);
+  const uint32_t item0 = blockIdx.x * (kThreads * kAppendItems) + threadIdx.x;
+  Spot s[kAppendItems];
+  uint4 x[kAppendItems][4];
+#pragma unroll
+  for (int n = 0; n < kAppendItems; ++n) {
+    s[n] = spot_of<D, true>(g, q, item0 + n * kThreads, D / 32);
+    if (s[n].held) {
+      const uint16_t *src = (s[n].value ? g.v + s[n].row * g.v_stride : g.k + s[n].row * g.k_stride) + s[n].head * D +
+                            s[n].part * 32;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        x[n][i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+    }
+  }
   const int page = 1 << g.t.page_shift;
-  uint32_t *codes = reinterpret_cast<uint32_t *>(s.block) + s.slot * (D / 8) + s.chunk;
-  codes[0] = kc;
-  codes[page * (D / 8)] = vc;
-  if (s.chunk % 4 == 0) {
-    uint32_t *params = reinterpret_cast<uint32_t *>(s.block) + page * (D / 4) + s.slot * (D / 32) + s.chunk / 4;
-    params[0] = kp;
-    params[page * (D / 32)] = vp;
+#pragma unroll
+  for (int n = 0; n < kAppendItems; ++n) {
+    if (!s[n].held)
+      continue;
+    uint32_t params;
+    const uint4 codes = quantise<BF16>(x[n], params);
+    const int slot = s[n].slot + (s[n].value ? page : 0);
+    *reinterpret_cast<uint4 *>(s[n].block + slot * (D / 2) + s[n].part * 16) = codes;
+    *reinterpret_cast<uint32_t *>(s[n].block + page * D + slot * (D / 8) + s[n].part * 4) = params;
   }
 }
 
 template <bool BF16> __device__ __forceinline__ uint4 restore8(uint32_t codes, uint32_t params) {
   const float scale = kv4_lo<BF16>(params), lo = kv4_hi<BF16>(params);
-  float x[8];
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) // 2^23 + c, exactly
-    x[i] = fmaf(__uint_as_float(0x4B000000u | ((codes >> (4 * i)) & 15u)) - 8388608.f, scale, lo);
-  return make_uint4(kv4_pack<BF16>(x[0], x[1]), kv4_pack<BF16>(x[2], x[3]), kv4_pack<BF16>(x[4], x[5]),
-                    kv4_pack<BF16>(x[6], x[7]));
-}
-
-template <int D, bool BF16> __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ CacheArgs g) {
-  pdl_begin();
-  const Spot s = spot_of<D>(g);
-  if (!s.live)
-    return;
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  if (s.held) {
-    const int page = 1 << g.t.page_shift;
-    const uint32_t *codes = reinterpret_cast<const uint32_t *>(s.block) + s.slot * (D / 8) + s.chunk;
-    const uint32_t *params =
-        reinterpret_cast<const uint32_t *>(s.block) + page * (D / 4) + s.slot * (D / 32) + s.chunk / 4;
-    const uint32_t kc = codes[0], vc = codes[page * (D / 8)], kp = params[0], vp = params[page * (D / 32)];
-    k = restore8<BF16>(kc, kp);
-    v = restore8<BF16>(vc, vp);
+  for (int i = 0; i < 4; ++i) {
+    // 2^23 + c less 2^23, exactly; scale * c is exact too.
+    const float2 c = add2(make_float2(__uint_as_float(0x4B000000u | ((codes >> (8 * i)) & 15u)),
+                                      __uint_as_float(0x4B000000u | ((codes >> (8 * i + 4)) & 15u))),
+                          make_float2(-8388608.f, -8388608.f));
+    const float2 x = add2(mul2(c, make_float2(scale, scale)), make_float2(lo, lo));
+    w[i] = kv4_pack<BF16>(x.x, x.y);
   }
-  const long long e = (s.row * g.kv_heads + s.head) * D + s.chunk * 8;
-  *reinterpret_cast<uint4 *>(g.ko + e) = k;
-  *reinterpret_cast<uint4 *>(g.vo + e) = v;
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int D, bool BF16> cudaError_t launch(const CacheArgs &g, bool append, cudaStream_t s) {
-  const long long work = static_cast<long long>(g.t.max_new) * g.kv_heads * (D / 8);
-  const dim3 grid(static_cast<unsigned>((work + kThreads - 1) / kThreads), g.t.batch);
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ CacheArgs g) {
+  pdl_begin();
+  const Kv4Seq q = kv4_seq(g.t, blockIdx.y);
+  const uint32_t item0 = blockIdx.x * (kThreads * kReadItems) + threadIdx.x;
+  const int page = 1 << g.t.page_shift;
+  Spot s[kReadItems];
+  uint32_t codes[kReadItems][2], params[kReadItems][2];
+#pragma unroll
+  for (int n = 0; n < kReadItems; ++n) {
+    s[n] = spot_of<D, false>(g, q, item0 + n * kThreads, D / 8);
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      codes[n][v] = params[n][v] = 0; // without a position: zeros
+      if (s[n].held) {
+        const int slot = s[n].slot + (v ? page : 0);
+        codes[n][v] = __ldg(reinterpret_cast<const uint32_t *>(s[n].block + slot * (D / 2) + s[n].part * 4));
+        params[n][v] =
+            __ldg(reinterpret_cast<const uint32_t *>(s[n].block + page * D + slot * (D / 8) + s[n].part / 4 * 4));
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < kReadItems; ++n)
+    if (s[n].live) {
+      const long long e = (s[n].row * g.kv_heads + s[n].head) * D + s[n].part * 8;
+      *reinterpret_cast<uint4 *>(g.ko + e) = restore8<BF16>(codes[n][0], params[n][0]);
+      *reinterpret_cast<uint4 *>(g.vo + e) = restore8<BF16>(codes[n][1], params[n][1]);
+    }
+}
+
+template <int D, bool BF16> cudaError_t launch(CacheArgs g, bool append, cudaStream_t s) {
+  const int of_token = g.kv_heads * (append ? 2 * D / 32 : D / 8);
+  const int per_block = kThreads * (append ? kAppendItems : kReadItems);
+  g.token_div = FastDiv(of_token);
+  const long long items = static_cast<long long>(g.t.max_new) * of_token;
+  const dim3 grid(static_cast<unsigned>((items + per_block - 1) / per_block), g.t.batch);
   return launch_pdl(append ? append_kernel<D, BF16> : read_kernel<D, BF16>, grid, kThreads, 0, s, g);
 }
 
 cudaError_t dispatch(const Kv4Cache &c, const CacheArgs &g, bool append, cudaStream_t s) {
-  // Chunks of a sequence's new tokens are counted in 32 bits.
-  if (static_cast<long long>(g.t.max_new) * c.kv_heads * (c.head_dim / 8) >= (1ll << 31) || g.t.batch > 65535)
+  // Items of a sequence's new tokens are counted in 31 bits.
+  if (static_cast<long long>(g.t.max_new) * c.kv_heads * (c.head_dim / 4) >= (1ll << 31) - (1 << 12) ||
+      g.t.batch > 65535)
     return cudaErrorInvalidValue;
   switch (c.head_dim * 2 + c.bf16) {
   case 64: return launch<32, false>(g, append, s);
@@ -183,7 +268,6 @@ cudaError_t kv4_append(const Kv4Cache &c, const Kv4Tokens &t, const void *k, lon
   g.k_stride = k_stride;
   g.v_stride = v_stride;
   g.kv_heads = c.kv_heads;
-  g.heads_div = FastDiv(c.kv_heads);
   return dispatch(c, g, true, stream);
 }
 
@@ -194,7 +278,6 @@ cudaError_t kv4_read(const Kv4Cache &c, const Kv4Tokens &t, void *k, void *v, cu
   g.ko = static_cast<uint16_t *>(k);
   g.vo = static_cast<uint16_t *>(v);
   g.kv_heads = c.kv_heads;
-  g.heads_div = FastDiv(c.kv_heads);
   return dispatch(c, g, false, stream);
 }
 
