@@ -56,7 +56,8 @@ struct RowsArgs {
   long long q_stride;
   int heads, kv_heads, group;
   int window, sinks;
-  float scale_log2; // softmax scale * log2(e)
+  float scale_log2; // |softmax scale| * log2(e)
+  uint32_t flip;    // sign of the scale, as a mask of two 16-bit values
   int b0, nb, rg0, nrg; // this launch's sequences and row groups
   int *counters;
   float *parts;
@@ -67,6 +68,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same from zero.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+               "{%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -157,12 +165,11 @@ struct Cursor {
 
 template <int D, int NT> struct RowsLayout {
   static constexpr int kStageBytes = kTile * (D + D / 4);
-  static constexpr int kStages = D == 128 && NT == 2 ? 3 : 4;
-  static constexpr int kCtasPerSm = D == 128 || NT == 2 ? 2 : 3;
+  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kCtasPerSm = NT == 1 ? 3 : 2;
   static constexpr int kMaxGrid = kCtasPerSm * 148;
   static constexpr int kRows = 8 * NT;
-  // Four warps' outputs, or the joining weights of every CTA's part.
-  static constexpr int kMergeFloats = kWarps * kRows * D > kMaxGrid * kRows ? kWarps * kRows * D : kMaxGrid * kRows;
+  static constexpr int kMergeFloats = kWarps / 2 * kRows * D; // outputs of half the warps
   static constexpr int kOffMerge = kStages * kStageBytes;
   static constexpr int kOffStats = kOffMerge + kMergeFloats * 4; // m, l per warp and row
   static constexpr int kOffBars = kOffStats + 2 * kWarps * kRows * 4;
@@ -349,6 +356,31 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
   // 16-byte chunk swizzle of a row of codes (see the tensor map).
   auto swz = [](int key) { return D == 128 ? (key >> 1) & 3 : D == 64 ? (key >> 2) & 1 : 0; };
   const int page_shift = g.t.page_shift, page = 1 << page_shift;
+  // Offsets in a stage of this lane's reads, the same for every tile.
+  uint32_t k_codes[2], k_groups[2], v_codes_a[2], v_codes_b[2], v_groups_a[2], v_groups_b[2];
+  uint32_t k_chunk[G];
+#pragma unroll
+  for (int c = 0; c < G; ++c)
+    k_chunk[c] = ((c ^ swz(key_row)) << 4) + 4 * lc;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int kk = warp * 32 + h * 16;
+    const int sub = kk >> page_shift, slot = kk & (page - 1);
+    const uint32_t codes = sbase + sub * page * D + slot * (D / 2);
+    const uint32_t groups = sbase + kTile * D + sub * page * (D / 4) + slot * (D / 8);
+    k_codes[h] = codes + key_row * (D / 2);
+    k_groups[h] = groups + key_row * (D / 8);
+    const int v_group = D == 128 ? lr >> 1 : D == 64 ? lr >> 2 : 0; // of this lane's channels
+    const uint32_t vc = codes + page * (D / 2), vg = groups + page * (D / 8) + v_group * 4;
+    auto v_chunk = [&](int key) {
+      return D == 128 ? ((v_group ^ swz(key)) << 4) + (lr & 1) * 8 : D == 64 ? ((v_group ^ swz(key)) << 4) + (lr & 3) * 4
+                                                                             : lr * 2;
+    };
+    v_codes_a[h] = vc + key_a * (D / 2) + v_chunk(key_a);
+    v_codes_b[h] = vc + key_b * (D / 2) + v_chunk(key_b);
+    v_groups_a[h] = vg + key_a * (D / 8);
+    v_groups_b[h] = vg + key_b * (D / 8);
+  }
   bool ok = true;
   int fill = 0;
   for (int t = t0; t < t1;) {
@@ -374,6 +406,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
 #pragma unroll
         for (int c = 0; c < G; ++c)
           w[c] = live ? *reinterpret_cast<const uint4 *>(p + c * 32) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < G; ++c)
+          w[c].x ^= g.flip, w[c].y ^= g.flip, w[c].z ^= g.flip, w[c].w ^= g.flip;
       }
 #pragma unroll
       for (int c = 0; c < G; ++c) {
@@ -387,7 +422,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
       // up = 2^(13 - floor(log2 most)), within fp32's normal range.
       const int ex = most > 0.f ? static_cast<int>(__float_as_uint(most) >> 23) : 127;
       const float up = __uint_as_float(static_cast<uint32_t>(min(max(267 - ex, 1), 254)) << 23);
-      const float down = __fdiv_rn(16777216.f, up) * g.scale_log2; // 2^24 / up
+      const float down = __fdiv_rn(16777216.f, up) * g.scale_log2; // 2^24 / up times the scale
 #pragma unroll
       for (int c = 0; c < G; ++c) {
         const uint32_t in[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
@@ -449,21 +484,17 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
         *abort = 1;
       }
       const int key0 = span.tile(cur.j) * kTile + warp * 32;
-      const uint32_t st = sbase + stage * L::kStageBytes;
+      const uint32_t st = stage * L::kStageBytes;
       // Whether every row sees all of this warp's keys.
       const bool clear = key0 + 31 <= x.pos_lo &&
                          (g.window <= 0 || key0 > x.pos_hi - g.window || key0 + 32 <= g.sinks);
       float s[2][NT][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int kk = warp * 32 + h * 16;
-        const int sub = kk >> page_shift, slot = kk & (page - 1);
-        const uint32_t codes = st + sub * page * D + slot * (D / 2);
-        const uint32_t params = st + kTile * D + sub * page * (D / 4) + slot * (D / 8);
-        const uint32_t row_a = codes + key_row * (D / 2), row_b = row_a + 8 * (D / 2);
+        const uint32_t row_a = st + k_codes[h];
         uint32_t pa[G], pb[G];
         {
-          const uint32_t at = params + key_row * (D / 8);
+          const uint32_t at = st + k_groups[h];
           if constexpr (G == 4) {
             const uint4 u = lds_v4(at), v = lds_v4(at + 8 * (D / 8));
             pa[0] = u.x, pa[1] = u.y, pa[2] = u.z, pa[3] = u.w;
@@ -478,14 +509,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
           }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s[h][nt][i] = 0.f;
-#pragma unroll
         for (int c = 0; c < G; ++c) {
-          const uint32_t off = ((c ^ swz(key_row)) << 4) + 4 * lc;
-          const uint32_t wa = lds_u32(row_a + off), wb = lds_u32(row_b + off);
+          const uint32_t wa = lds_u32(row_a + k_chunk[c]), wb = lds_u32(row_a + k_chunk[c] + 8 * (D / 2));
           const uint32_t lo[4] = {wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u};
           const uint32_t ya = wa >> 8, yb = wb >> 8;
           const uint32_t hi[4] = {ya & 0x000F000Fu, yb & 0x000F000Fu, ya & 0x00F000F0u, yb & 0x00F000F0u};
@@ -493,24 +518,29 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
           const float sb = kv4_lo<BF16>(pb[c]), mb = kv4_hi<BF16>(pb[c]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16(acc, lo, qf[nt][c][0], qf[nt][c][1]);
+            float acc[4];
+            mma_f16_first(acc, lo, qf[nt][c][0], qf[nt][c][1]);
             mma_f16(acc, hi, qf[nt][c][2], qf[nt][c][3]);
-            s[h][nt][0] += acc[0] * sa + qsum[nt][c][0] * ma;
-            s[h][nt][1] += acc[1] * sa + qsum[nt][c][1] * ma;
-            s[h][nt][2] += acc[2] * sb + qsum[nt][c][0] * mb;
-            s[h][nt][3] += acc[3] * sb + qsum[nt][c][1] * mb;
+            float(&x)[4] = s[h][nt];
+            if (c == 0) {
+              x[0] = qsum[nt][0][0] * ma;
+              x[1] = qsum[nt][0][1] * ma;
+              x[2] = qsum[nt][0][0] * mb;
+              x[3] = qsum[nt][0][1] * mb;
+            } else {
+              x[0] = fmaf(qsum[nt][c][0], ma, x[0]);
+              x[1] = fmaf(qsum[nt][c][1], ma, x[1]);
+              x[2] = fmaf(qsum[nt][c][0], mb, x[2]);
+              x[3] = fmaf(qsum[nt][c][1], mb, x[3]);
+            }
+            x[0] = fmaf(acc[0], sa, x[0]);
+            x[1] = fmaf(acc[1], sa, x[1]);
+            x[2] = fmaf(acc[2], sb, x[2]);
+            x[3] = fmaf(acc[3], sb, x[3]);
           }
         }
       }
-      // Scores in powers of two; what a row does not see is replaced.
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s[h][nt][i] *= factor[nt][i & 1];
+      // What a row does not see is replaced.
       if (!clear) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -530,7 +560,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          top[nt][i] = fmaxf(fmaxf(s[0][nt][i], s[0][nt][i + 2]), fmaxf(s[1][nt][i], s[1][nt][i + 2]));
+          // In powers of two; the factor is positive.
+          top[nt][i] =
+              factor[nt][i] * fmaxf(fmaxf(s[0][nt][i], s[0][nt][i + 2]), fmaxf(s[1][nt][i], s[1][nt][i + 2]));
           raise = raise || top[nt][i] > m[nt][i] + 8.f;
         }
       if (__any_sync(~0u, raise)) {
@@ -556,11 +588,12 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         // Nothing seen yet: every score is -inf, and so must its power be 0.
-        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+        const float m0 = m[nt][0] == -INFINITY ? 0.f : -m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : -m[nt][1];
+        const float f0 = factor[nt][0], f1 = factor[nt][1];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float p0 = ex2_ftz(s[h][nt][0] - m0), p1 = ex2_ftz(s[h][nt][1] - m1);
-          const float p2 = ex2_ftz(s[h][nt][2] - m0), p3 = ex2_ftz(s[h][nt][3] - m1);
+          const float p0 = ex2_ftz(fmaf(s[h][nt][0], f0, m0)), p1 = ex2_ftz(fmaf(s[h][nt][1], f1, m1));
+          const float p2 = ex2_ftz(fmaf(s[h][nt][2], f0, m0)), p3 = ex2_ftz(fmaf(s[h][nt][3], f1, m1));
           l[nt][0] += p0 + p2;
           l[nt][1] += p1 + p3;
           pf[h][nt][0] = transpose8x8(kv4_pack<BF16>(p0, p1));
@@ -569,17 +602,12 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int kk = warp * 32 + h * 16;
-        const int sub = kk >> page_shift, slot = kk & (page - 1);
-        const uint32_t codes = st + sub * page * D + page * (D / 2) + slot * (D / 2);
-        const uint32_t params = st + kTile * D + sub * page * (D / 4) + page * (D / 8) + slot * (D / 8) +
-                                (D == 128 ? lr >> 1 : D == 64 ? lr >> 2 : 0) * 4;
         // Channel rows lr and lr + 8 of every tile; the keys of both pairs.
         uint32_t scale[2], low[2], w[2][2][D == 128 ? 2 : 1];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int ka = key_a + 8 * u, kb = key_b + 8 * u;
-          uint32_t pa = lds_u32(params + ka * (D / 8)), pb = lds_u32(params + kb * (D / 8));
+          uint32_t pa = lds_u32(st + v_groups_a[h] + 8 * u * (D / 8)), pb = lds_u32(st + v_groups_b[h] + 8 * u * (D / 8));
           if (!clear) {
             const int key = key0 + h * 16;
             pa = key + ka < x.s.len ? pa : 0u;
@@ -587,18 +615,17 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
           }
           scale[u] = __byte_perm(pa, pb, 0x5410);
           low[u] = __byte_perm(pa, pb, 0x7632);
-          const uint32_t ra = codes + ka * (D / 2), rb = codes + kb * (D / 2);
+          const uint32_t ra = st + v_codes_a[h] + 8 * u * (D / 2), rb = st + v_codes_b[h] + 8 * u * (D / 2);
           if constexpr (D == 128) {
-            const uint2 a = lds_v2(ra + (((lr >> 1) ^ swz(key_a)) << 4) + (lr & 1) * 8);
-            const uint2 c = lds_v2(rb + (((lr >> 1) ^ swz(key_b)) << 4) + (lr & 1) * 8);
+            const uint2 a = lds_v2(ra), c = lds_v2(rb);
             w[u][0][0] = a.x, w[u][0][1] = a.y;
             w[u][1][0] = c.x, w[u][1][1] = c.y;
           } else if constexpr (D == 64) {
-            w[u][0][0] = lds_u32(ra + (((lr >> 2) ^ swz(key_a)) << 4) + (lr & 3) * 4);
-            w[u][1][0] = lds_u32(rb + (((lr >> 2) ^ swz(key_b)) << 4) + (lr & 3) * 4);
+            w[u][0][0] = lds_u32(ra);
+            w[u][1][0] = lds_u32(rb);
           } else {
-            w[u][0][0] = lds_u16(ra + lr * 2);
-            w[u][1][0] = lds_u16(rb + lr * 2);
+            w[u][0][0] = lds_u16(ra);
+            w[u][1][0] = lds_u16(rb);
           }
         }
         if constexpr (D == 32) {
@@ -660,30 +687,38 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
         }
       }
     consumer_barrier();
+    // Warps 2 and 3 leave theirs, warps 0 and 1 add their own to it.
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int half = 1; half >= 0; --half) {
+      if (warp / 2 == half) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = nt * 8 + 2 * lc + i;
-        float top = stat_m[row];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w)
-          top = fmaxf(top, stat_m[w * kRows + row]);
-        const float r = m[nt][i] == -INFINITY ? 0.f : ex2_ftz(m[nt][i] - top);
-        // This thread's channels of the row are D / 8 neighbours.
-        float *dst = merge + (warp * kRows + row) * D + lr * (D / 8);
-        float v[D / 8];
+          for (int i = 0; i < 2; ++i) {
+            const int row = nt * 8 + 2 * lc + i;
+            float top = stat_m[row];
 #pragma unroll
-        for (int d = 0; d < kTiles; ++d) {
-          const int at = D == 32 ? d : (d / 4) * 8 + d % 4;
-          v[at] = o[d][nt][i] * r;
-          v[at + (D == 32 ? 2 : 4)] = o[d][nt][i + 2] * r;
-        }
+            for (int w = 1; w < kWarps; ++w)
+              top = fmaxf(top, stat_m[w * kRows + row]);
+            const float r = m[nt][i] == -INFINITY ? 0.f : ex2_ftz(m[nt][i] - top);
+            // This thread's channels of the row are D / 8 neighbours.
+            float4 *dst = reinterpret_cast<float4 *>(merge + ((warp & 1) * kRows + row) * D + lr * (D / 8));
+            float v[D / 8];
 #pragma unroll
-        for (int c = 0; c < D / 8; c += 4)
-          *reinterpret_cast<float4 *>(dst + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+            for (int d = 0; d < kTiles; ++d) {
+              const int at = D == 32 ? d : (d / 4) * 8 + d % 4;
+              v[at] = o[d][nt][i] * r;
+              v[at + (D == 32 ? 2 : 4)] = o[d][nt][i + 2] * r;
+            }
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              const float4 y = half ? make_float4(0.f, 0.f, 0.f, 0.f) : dst[c];
+              dst[c] = make_float4(y.x + v[4 * c], y.y + v[4 * c + 1], y.z + v[4 * c + 2], y.w + v[4 * c + 3]);
+            }
+          }
       }
-    consumer_barrier();
+      consumer_barrier();
+    }
     const bool whole = from_start && to_end;
     // A CTA leaves at most two parts: of the unit it came in on and of the
     // one it goes out on.
@@ -701,11 +736,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
     for (int it = tid; it < kRows * D / 4; it += 32 * kWarps) {
       const int row = it / (D / 4), d = it % (D / 4) * 4;
       float4 v = *reinterpret_cast<const float4 *>(merge + row * D + d);
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) {
-        const float4 y = *reinterpret_cast<const float4 *>(merge + (w * kRows + row) * D + d);
-        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
-      }
+      const float4 y = *reinterpret_cast<const float4 *>(merge + (kRows + row) * D + d);
+      v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
       float top = stat_m[row];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w)
@@ -728,31 +760,36 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
     if (!whole) {
       // ---- the last CTA to finish joins the unit's parts
       const int first = cur.base / quota, parts = (cur.base + cur.cnt - 1) / quota - first + 1;
-      __threadfence();
       consumer_barrier();
       if (tid == 0) {
         int *c = g.counters + cur.e * g.kv_heads + cur.h;
+        __threadfence(); // the CTA's part, written before the barrier
         const int seen = atomicAdd(c, 1);
+        __threadfence();
         *is_last = seen == parts - 1;
         if (seen == parts - 1)
           *c = 0;
       }
       consumer_barrier();
       if (*is_last) {
-        __threadfence();
         auto part_of = [&](int i) {
           // The unit's first CTA went out on it unless the unit starts there.
           const int cta = first + i;
           const bool began = cur.base >= cta * quota;
           return g.parts + static_cast<long long>(cta * 2 + (began ? 1 : 0)) * kPartFloats;
         };
-        for (int i = tid; i < parts * kRows; i += 32 * kWarps)
-          merge[i] = __ldcg(part_of(i / kRows) + kRows * D + i % kRows);
+        // Largest maximum of each row, by 32 kWarps / kRows threads each.
+        float best = -INFINITY;
+#pragma unroll 4
+        for (int i = tid / kRows; i < parts; i += 32 * kWarps / kRows)
+          best = fmaxf(best, __ldcg(part_of(i) + kRows * D + tid % kRows));
+        merge[tid] = best;
         consumer_barrier();
         for (int it = tid; it < kRows * D / 4; it += 32 * kWarps) {
           const int row = it / (D / 4), d = it % (D / 4) * 4;
-          float top = -INFINITY;
-          for (int i = 0; i < parts; ++i)
+          float top = merge[row];
+#pragma unroll
+          for (int i = 1; i < 32 * kWarps / kRows; ++i)
             top = fmaxf(top, merge[i * kRows + row]);
           float sum = 0.f;
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -760,8 +797,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
           for (int i = 0; i < parts; ++i) {
             const float *p = part_of(i);
             const float4 y = __ldcg(reinterpret_cast<const float4 *>(p + row * D + d));
-            const float ly = __ldcg(p + kRows * D + kRows + row);
-            const float my = merge[i * kRows + row];
+            const float my = __ldcg(p + kRows * D + row), ly = __ldcg(p + kRows * D + kRows + row);
             const float r = my == -INFINITY ? 0.f : ex2_ftz(my - top);
             sum += ly * r;
             v.x += y.x * r, v.y += y.y * r, v.z += y.z * r, v.w += y.w * r;
@@ -809,7 +845,9 @@ cudaError_t kv4_attend_rows(const Kv4Cache &c, const Kv4Tokens &t, const Kv4Atte
   g.group_div = FastDiv(g.group);
   g.window = a.window;
   g.sinks = a.sinks;
-  g.scale_log2 = a.scale * kLog2e;
+  // Not 0: hidden scores are -inf before the scale is applied.
+  g.scale_log2 = std::max(fabsf(a.scale) * kLog2e, 1e-30f);
+  g.flip = a.scale < 0.f ? 0x80008000u : 0u;
   g.counters = static_cast<int *>(a.workspace);
   g.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(a.workspace) + static_cast<size_t>(kMaxUnits) * 4);
   const int D = c.head_dim, P = c.page_size;
