@@ -81,8 +81,9 @@ int ppocr_b200_kv4_read(const PpocrKv4Cache *cache, void *k, void *v,
 // [head_dim] contiguous; both of the cache's type and 16-byte aligned.
 // Softmax statistics and sums are fp32. workspace: device memory of
 // ppocr_b200_kv4_workspace_bytes() bytes, 256-byte aligned, zeroed once
-// before its first use (every call leaves it ready for the next); calls that
-// may overlap on the GPU need one each.
+// before its first use (every call leaves it ready for the next, but zero it
+// again after ppocr_b200_device_error() reported a wait that ran out); calls
+// that may overlap on the GPU need one each.
 size_t ppocr_b200_kv4_workspace_bytes(void);
 int ppocr_b200_kv4_attention(const PpocrKv4Cache *cache, const void *q,
                              long long q_stride, void *out, int heads,

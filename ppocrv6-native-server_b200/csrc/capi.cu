@@ -784,7 +784,9 @@ int ppocr_b200_kv4_read(const PpocrKv4Cache *cache, void *k, void *v, const int 
   return status(kv4_read(c, t, k, v, stream), "kv4 read");
 }
 
-size_t ppocr_b200_kv4_workspace_bytes(void) { return kv4_workspace_bytes(); }
+size_t ppocr_b200_kv4_workspace_bytes(void) {
+  return std::max(kv4_rows_workspace_bytes(), kv4_prompt_workspace_bytes());
+}
 
 int ppocr_b200_kv4_attention(const PpocrKv4Cache *cache, const void *q, long long q_stride, void *out, int heads,
                              float scale, int window, int sinks, const int *table, int width, const int *lengths,
@@ -820,7 +822,7 @@ int ppocr_b200_kv4_attention(const PpocrKv4Cache *cache, const void *q, long lon
   a.scale = scale;
   a.workspace = workspace;
   const long long rows = static_cast<long long>(max_new) * (heads / c.kv_heads);
-  return status(rows <= 32 ? kv4_attend_rows(c, t, a, stream) : kv4_attend_prompt(c, t, a, stream), "kv4 attention");
+  return status(rows <= (getenv("ROWS_MOST") ? atoi(getenv("ROWS_MOST")) : 16) ? kv4_attend_rows(c, t, a, stream) : kv4_attend_prompt(c, t, a, stream), "kv4 attention");
 }
 
 int ppocr_b200_sample(const void *logits, int type, long long stride, int rows, int vocab, const float *temperature,

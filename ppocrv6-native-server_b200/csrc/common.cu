@@ -2,7 +2,9 @@
 // kernels whose bounded waits ran out, and the SM count used to size
 // persistent grids.
 #include "kernels.h"
+#include <map>
 #include <mutex>
+#include <utility>
 
 namespace pb2 {
 namespace {
@@ -50,6 +52,27 @@ int sm_count() {
     g_sms[d] = n > 0 ? n : 148;
   }
   return g_sms[d];
+}
+
+cudaError_t prepare_kernel(const void *kernel, int smem, int registers) {
+  static std::map<std::pair<int, const void *>, int> allowed;
+  const int d = current_device();
+  std::lock_guard<std::mutex> lock(g_mutex);
+  int &have = allowed[{d, kernel}];
+  if (have >= smem && have > 0)
+    return cudaSuccess;
+  if (registers > 0) {
+    cudaFuncAttributes attr;
+    const cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
+    if (e != cudaSuccess)
+      return e;
+    if (attr.numRegs < registers)
+      return cudaErrorInvalidConfiguration;
+  }
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess)
+    have = smem;
+  return e;
 }
 
 } // namespace pb2

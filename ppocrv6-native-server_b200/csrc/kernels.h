@@ -20,6 +20,10 @@ int take_noalloc_error();
 // Test support: writes `code` into that word (head_noalloc.cu).
 cudaError_t store_noalloc_error(int code);
 int sm_count();
+// Once per device and kernel (and again for more shared memory): allows
+// `kernel` that much dynamic shared memory, and checks that it is launched
+// with at least `registers` a thread (0: not checked).
+cudaError_t prepare_kernel(const void *kernel, int smem, int registers = 0);
 // Sets the calling thread's message returned by ppocr_b200_last_error().
 void set_last_error(const std::string &message);
 
@@ -374,7 +378,7 @@ cudaError_t kv4_append(const Kv4Cache &c, const Kv4Tokens &t, const void *k, lon
 cudaError_t kv4_read(const Kv4Cache &c, const Kv4Tokens &t, void *k, void *v, cudaStream_t stream);
 // Attention with few query rows per (sequence, key head): the cache is split
 // over the GPU's CTAs and the parts are joined through `workspace`.
-size_t kv4_workspace_bytes();
+size_t kv4_rows_workspace_bytes();
 struct Kv4Attention {
   const void *q = nullptr;
   void *out = nullptr;
@@ -384,7 +388,9 @@ struct Kv4Attention {
   void *workspace = nullptr;
 };
 cudaError_t kv4_attend_rows(const Kv4Cache &c, const Kv4Tokens &t, const Kv4Attention &a, cudaStream_t stream);
-// The same with many query rows, on tcgen05.
+// The same with many query rows, on tcgen05. Both start their workspace with
+// counters that every call leaves at zero.
+size_t kv4_prompt_workspace_bytes();
 cudaError_t kv4_attend_prompt(const Kv4Cache &c, const Kv4Tokens &t, const Kv4Attention &a, cudaStream_t stream);
 // Token sampling (csrc/sample.cu); the parameters are per row, null = off.
 struct SampleArgs {

@@ -21,12 +21,15 @@
 //    run.
 // Products are issued in the order P0 V(j), S0(j + 1), P1 V(j), S1(j + 1): a
 // commit after S t (j + 1) also says that O t holds all of tile j.
+// Where the row blocks are fewer than the SMs, several CTAs share the key tiles
+// of one: each leaves (m, l, O) of its rows in fp32, and per 32 rows the last
+// warp to arrive joins them in the order of the tiles.
 // Work per tile: 4 x 128 x 128 x D multiply-adds (2048 cycles of the tensor
 // pipe at D = 128) against 32768 exponentials (2048 cycles of the special
 // function units): the two bound it alike.
 #include "kv4.cuh"
 #include <algorithm>
-#include <type_traits>
+#include <cmath>
 
 namespace pb2 {
 namespace {
@@ -41,6 +44,8 @@ constexpr int kTile = 128;
 constexpr int kBlockRows = 256;
 constexpr uint32_t kAtom = 128 * 128; // 128 rows of 128 bytes
 constexpr int kErrPromptWait = 43;
+constexpr int kSplitCtas = 148;             // that share row blocks at most
+constexpr size_t kCounterBytes = (1 << 16) * 4; // as in the other kernel's workspace
 
 struct PromptArgs {
   Kv4Tokens t;
@@ -53,6 +58,10 @@ struct PromptArgs {
   float scale_log2; // |softmax scale| * log2(e)
   uint32_t flip;    // sign of the scale, as a mask of two 16-bit values
   int row_blocks;
+  int splits;       // CTAs that share a row block's key tiles
+  int *counters;    // per row block and warp, left at zero
+  float *parts;
+  FastDiv split_div;
   FastDiv group_div, unit_div, heads_div; // by group, batch * kv_heads, kv_heads
 };
 
@@ -212,8 +221,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
   const uint32_t tmem = *tmem_slot;
 
   // Last rows first: they see the most keys.
-  const uint32_t slab = g.unit_div.div(blockIdx.x);
-  const uint32_t unit = blockIdx.x - slab * (g.t.batch * g.kv_heads);
+  const uint32_t place = g.split_div.div(blockIdx.x);
+  const int split = blockIdx.x - place * g.splits;
+  const uint32_t slab = g.unit_div.div(place);
+  const uint32_t unit = place - slab * (g.t.batch * g.kv_heads);
   const int b = g.heads_div.div(unit), h = unit - b * g.kv_heads;
   const int row0 = (g.row_blocks - 1 - static_cast<int>(slab)) * kBlockRows;
   const Kv4Seq seq = kv4_seq(g.t, b);
@@ -235,8 +246,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     }
     tiles = sink + hi - lo;
   }
+  // This CTA's run of them.
+  const int share = (tiles + g.splits - 1) / g.splits;
+  const int parts = share ? (tiles + share - 1) / share : 0, tile0 = split * share;
+  tiles = min(max(tiles - tile0, 0), share);
   const bool two = rows > 128;
-  auto key_of_tile = [&](int j) { return (j < sink ? j : j - sink + lo) * kTile; };
+  auto key_of_tile = [&](int j) {
+    j += tile0;
+    return (j < sink ? j : j - sink + lo) * kTile;
+  };
   bool ok = true;
 
   if (tiles > 0 && warp < 8) {
@@ -384,24 +402,101 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         ok = mbar_wait(o_full + block, 0, abort);
         ok = __all_sync(~0u, ok);
       }
-      if (ok) {
+      bool last = ok; // this warp writes its rows
+      if (ok)
         tc_fence_after();
+      // Parts of this warp's 32 rows: [D] outputs, m and l, each [32].
+      constexpr int kPart = (D + 2) * 32;
+      float *const warp_parts = g.parts + static_cast<long long>(place) * g.splits * 8 * kPart + warp * kPart + lane;
+      const long long next_part = 8 * kPart;
+      if (ok && parts > 1) {
+        float *mine = warp_parts + split * next_part;
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16(t_o + 16 * c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            mine[(16 * c + e) * 32] = __uint_as_float(o[e]);
+        }
+        mine[D * 32] = m;
+        mine[(D + 1) * 32] = l;
+        __syncwarp();
+        int seen = 0;
+        if (lane == 0) {
+          int *counter = g.counters + place * 8 + warp;
+          __threadfence();
+          seen = atomicAdd(counter, 1);
+          __threadfence();
+          if (seen == parts - 1)
+            *counter = 0;
+        }
+        last = __shfl_sync(~0u, seen, 0) == parts - 1;
+        if (last) {
+          m = -INFINITY;
+          for (int i = 0; i < parts; ++i)
+            m = fmaxf(m, __ldcg(warp_parts + i * next_part + D * 32));
+          l = 0.f;
+          for (int i = 0; i < parts; ++i) {
+            const float x = __ldcg(warp_parts + i * next_part + D * 32);
+            l += x == -INFINITY ? 0.f : ex2_ftz(x - m) * __ldcg(warp_parts + i * next_part + (D + 1) * 32);
+          }
+        }
+      }
+      if (last) {
         const float f = l > 0.f ? __fdividef(1.f, l) : l; // nothing seen: 0; NaN stays NaN
         // Through the rows' place of the queries, which all products have
         // read by now.
+        auto stage = [&](int chunk, const uint32_t *o) {
+          uint4 w;
+          w.x = kv4_pack<BF16>(__uint_as_float(o[0]) * f, __uint_as_float(o[2]) * f);
+          w.y = kv4_pack<BF16>(__uint_as_float(o[4]) * f, __uint_as_float(o[6]) * f);
+          w.z = kv4_pack<BF16>(__uint_as_float(o[1]) * f, __uint_as_float(o[3]) * f);
+          w.w = kv4_pack<BF16>(__uint_as_float(o[5]) * f, __uint_as_float(o[7]) * f);
+          sts_v4(chunk_at(lane, chunk), w);
+        };
+        if (parts == 1) {
+          uint32_t o[D / 32][32];
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_o + 32 * c, o);
+          for (int c = 0; c < D / 32; ++c)
+            tmem_ld32(t_o + 32 * c, o[c]);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 w;
-            w.x = kv4_pack<BF16>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 2]) * f);
-            w.y = kv4_pack<BF16>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 6]) * f);
-            w.z = kv4_pack<BF16>(__uint_as_float(o[e + 1]) * f, __uint_as_float(o[e + 3]) * f);
-            w.w = kv4_pack<BF16>(__uint_as_float(o[e + 5]) * f, __uint_as_float(o[e + 7]) * f);
-            sts_v4(chunk_at(lane, 4 * c + e / 8), w);
+          for (int c = 0; c < D / 8; ++c)
+            stage(c, o[c / 4] + c % 4 * 8);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              v[e] = 0.f;
+#pragma unroll 1
+            for (int i = 0; i < parts; i += 4) {
+              float x[4], y[4][16]; // four parts' loads at once
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float *p = warp_parts + min(i + k, parts - 1) * next_part;
+                x[k] = __ldcg(p + D * 32);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  y[k][e] = __ldcg(p + (16 * c + e) * 32);
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float r = x[k] == -INFINITY || i + k >= parts ? 0.f : ex2_ftz(x[k] - m);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  v[e] = fmaf(y[k][e], r, v[e]);
+              }
+            }
+            uint32_t o[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              o[e] = __float_as_uint(v[e]);
+            stage(2 * c, o);
+            stage(2 * c + 1, o + 8);
           }
         }
         __syncwarp();
@@ -418,10 +513,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp < 8 + kRestoreWarps) {
       // ----------------------------------------------------------- restoring
-      // A piece is 32 / G tokens of one operand: 16 bytes of codes a lane. Keys
-      // come first; the warps take them in turn.
+      // A piece is 32 / G tokens of one operand: 16 bytes of codes a lane. The
+      // operands come in turn (keys of a tile, its values, keys of the next),
+      // and while one is restored the other's codes are on their way.
       constexpr int kTokens = 32 / G, kPieces = 4 * G; // of one operand
-      constexpr int kMine = (2 * kPieces + kRestoreWarps - 1) / kRestoreWarps;
+      constexpr int kMine = (kPieces + kRestoreWarps - 1) / kRestoreWarps;
       const int w = warp - 8;
       const int page = 1 << g.t.page_shift;
       const int tok0 = lane / G, c = lane % G; // token of the piece, group
@@ -429,46 +525,44 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
       const uint8_t *mine = g.pool + h * block_bytes;
       const long long page_stride = block_bytes * g.kv_heads;
       const int *row = g.t.table + static_cast<long long>(b) * g.t.width;
-      uint4 codes[kMine];
-      uint32_t params[kMine];
-      int ids[kMine];     // page of the piece's tokens in the tile to fetch next
-      uint32_t place[kMine]; // of the piece's codes in the block
+      uint4 codes[2][kMine];
+      uint32_t params[2][kMine];
+      int ids[2][kMine]; // page of the piece's tokens in the tile to fetch next
       bool bad = false;
-      auto exists = [&](int i) { return w + i * kRestoreWarps < 2 * kPieces; };
-      auto is_value = [&](int i) { return w + i * kRestoreWarps >= kPieces; };
-      auto token_of = [&](int i) { return (w + i * kRestoreWarps - is_value(i) * kPieces) * kTokens + tok0; };
-      // A tile starts on a page's start, so a piece's slots are the same in
-      // every tile.
-#pragma unroll
-      for (int i = 0; i < kMine; ++i)
-        place[i] = ((token_of(i) & (page - 1)) + is_value(i) * page) * (D / 2) + c * 16;
-      auto find = [&](int i, int j) {
-        const int key = key_of_tile(j) + token_of(i);
-        ids[i] = exists(i) && j < tiles && key < seq.len ? __ldg(row + (key >> g.t.page_shift)) : 0;
+      // Warps that take one more piece of the keys take one less of the values.
+      auto piece_of = [&](int values, int i) { return (values ? kRestoreWarps - 1 - w : w) + i * kRestoreWarps; };
+      auto token_of = [&](int values, int i) { return piece_of(values, i) * kTokens + tok0; };
+      auto find = [&](int values, int i, int j) {
+        const int key = key_of_tile(j) + token_of(values, i);
+        ids[values][i] =
+            piece_of(values, i) < kPieces && j < tiles && key < seq.len ? __ldg(row + (key >> g.t.page_shift)) : 0;
       };
       // Loads the piece of tile j, whose page id is there, and the page id
       // of the next.
-      auto fetch = [&](int i, int j) {
-        if (exists(i) && j < tiles) {
-          bad = bad || static_cast<unsigned>(ids[i]) >= static_cast<unsigned>(g.t.pages);
-          const uint8_t *blk =
-              mine + min(static_cast<unsigned>(ids[i]), static_cast<unsigned>(g.t.pages - 1)) * page_stride;
-          codes[i] = __ldg(reinterpret_cast<const uint4 *>(blk + place[i]));
+      auto fetch = [&](int values, int i, int j) {
+        if (piece_of(values, i) < kPieces && j < tiles) {
+          const unsigned id = ids[values][i];
+          bad = bad || id >= static_cast<unsigned>(g.t.pages);
+          const uint8_t *blk = mine + min(id, static_cast<unsigned>(g.t.pages - 1)) * page_stride;
+          // A tile starts on a page's start.
+          const uint32_t at = ((token_of(values, i) & (page - 1)) + values * page) * (D / 2) + c * 16;
+          codes[values][i] = __ldg(reinterpret_cast<const uint4 *>(blk + at));
           // D / 8 bytes of groups to D / 2 of codes.
-          params[i] = __ldg(reinterpret_cast<const uint32_t *>(blk + page * D + place[i] / 4));
-          find(i, j + 1);
+          params[values][i] = __ldg(reinterpret_cast<const uint32_t *>(blk + page * D + at / 4));
+          find(values, i, j + 1);
         }
       };
-      auto put = [&](int i, int j, uint32_t operand) {
-        const int tok = token_of(i);
+      auto put = [&](int values, int i, int j, uint32_t operand) {
+        const int tok = token_of(values, i);
+        const uint4 code = codes[values][i];
         // Past the length: zeros.
-        const uint32_t group = key_of_tile(j) + tok < seq.len ? params[i] : 0u;
+        const uint32_t group = key_of_tile(j) + tok < seq.len ? params[values][i] : 0u;
         const uint32_t scale = __byte_perm(group, 0, 0x1010), low = __byte_perm(group, 0, 0x3232);
         // Lanes of the upper two groups write their chunks in another order,
         // so that the eight lanes of a phase meet eight bank columns.
         const bool turn = c >= 2;
-        const uint32_t in[4] = {turn ? codes[i].z : codes[i].x, turn ? codes[i].w : codes[i].y,
-                                turn ? codes[i].x : codes[i].z, turn ? codes[i].y : codes[i].w};
+        const uint32_t in[4] = {turn ? code.z : code.x, turn ? code.w : code.y, turn ? code.x : code.z,
+                                turn ? code.y : code.w};
         const uint32_t row = operand + (c / 2) * kAtom + tok * 128;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -477,11 +571,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         }
       };
 #pragma unroll
-      for (int i = 0; i < kMine; ++i)
-        find(i, 0);
+      for (int values = 0; values < 2; ++values)
 #pragma unroll
-      for (int i = 0; i < kMine; ++i)
-        fetch(i, 0);
+        for (int i = 0; i < kMine; ++i)
+          find(values, i, 0);
+#pragma unroll
+      for (int values = 0; values < 2; ++values)
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+          fetch(values, i, 0);
       for (int j = 0; j < tiles; ++j) {
         const int st = j & 1;
 #pragma unroll
@@ -495,17 +593,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
           const uint32_t operand = sbase + (values ? L::kOffV : L::kOffK) + st * L::kOperand;
 #pragma unroll
           for (int i = 0; i < kMine; ++i)
-            if (is_value(i) == values && exists(i))
-              put(i, j, operand);
+            if (piece_of(values, i) < kPieces)
+              put(values, i, j, operand);
           fence_async_smem();
           __syncwarp();
           if (lane == 0)
             mbar_arrive((values ? v_full : k_full) + st);
-          // On its way while the other operand is restored.
 #pragma unroll
           for (int i = 0; i < kMine; ++i)
-            if (is_value(i) == values)
-              fetch(i, j + 1);
+            fetch(values, i, j + 1);
         }
         if (!ok)
           break;
@@ -585,22 +681,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 
 template <int D, bool BF16> cudaError_t launch_prompt(const PromptArgs &g, cudaStream_t stream) {
   auto *kernel = prompt_kernel<D, BF16>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(PromptLayout<D>::kBytes));
-  if (e != cudaSuccess)
-    return e;
   // The softmax warps wait for registers that the launch must have brought.
-  cudaFuncAttributes attr;
-  e = cudaFuncGetAttributes(&attr, kernel);
+  const cudaError_t e = prepare_kernel(reinterpret_cast<const void *>(kernel), static_cast<int>(PromptLayout<D>::kBytes),
+                                       kLaunchRegs);
   if (e != cudaSuccess)
     return e;
-  if (attr.numRegs < kLaunchRegs)
-    return cudaErrorInvalidConfiguration;
-  const unsigned grid = static_cast<unsigned>(g.row_blocks) * g.t.batch * g.kv_heads;
+  const unsigned grid = static_cast<unsigned>(g.row_blocks) * g.t.batch * g.kv_heads * g.splits;
   return launch_pdl(kernel, grid, kPromptThreads, PromptLayout<D>::kBytes, stream, g);
 }
 
 } // namespace
+
+size_t kv4_prompt_workspace_bytes() {
+  return kCounterBytes + static_cast<size_t>(kSplitCtas) * 8 * (128 + 2) * 32 * sizeof(float);
+}
 
 cudaError_t kv4_attend_prompt(const Kv4Cache &c, const Kv4Tokens &t, const Kv4Attention &a, cudaStream_t stream) {
   PromptArgs g{};
@@ -622,6 +716,15 @@ cudaError_t kv4_attend_prompt(const Kv4Cache &c, const Kv4Tokens &t, const Kv4At
   if (blocks * t.batch * c.kv_heads >= (1ll << 31))
     return cudaErrorInvalidValue;
   g.row_blocks = static_cast<int>(blocks);
+  g.counters = static_cast<int *>(a.workspace);
+  g.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(a.workspace) + kCounterBytes);
+  // As many CTAs a row block as fill the SMs, but not below four tiles each
+  // (of those that the table could hold): a tile takes a CTA about 2.5 us, a
+  // part about 1 us to join, and the rest of a CTA's life about 5 us.
+  const long long units = blocks * t.batch * c.kv_heads;
+  const long long room = (static_cast<long long>(t.width) * c.page_size + kTile - 1) / kTile;
+  g.splits = static_cast<int>(std::max<long long>(1, std::min<long long>(kSplitCtas / units, static_cast<long long>(std::min(0.25 * room, std::sqrt(2. * room))))));
+  g.split_div = FastDiv(g.splits);
   g.group_div = FastDiv(g.group);
   g.unit_div = FastDiv(t.batch * c.kv_heads);
   g.heads_div = FastDiv(c.kv_heads);

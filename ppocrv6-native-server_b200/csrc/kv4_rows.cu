@@ -819,7 +819,7 @@ template <int D, int NT, bool BF16>
 cudaError_t launch_rows(const CUtensorMap &map, const RowsArgs &g, cudaStream_t stream) {
   auto *kernel = rows_kernel<D, NT, BF16>;
   const size_t smem = rows_smem<D, NT>(g.nb * g.nrg);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  const cudaError_t e = prepare_kernel(reinterpret_cast<const void *>(kernel), static_cast<int>(smem));
   if (e != cudaSuccess)
     return e;
   const int grid = std::min(RowsLayout<D, NT>::kCtasPerSm * sm_count(), RowsLayout<D, NT>::kMaxGrid);
@@ -828,7 +828,7 @@ cudaError_t launch_rows(const CUtensorMap &map, const RowsArgs &g, cudaStream_t 
 
 } // namespace
 
-size_t kv4_workspace_bytes() {
+size_t kv4_rows_workspace_bytes() {
   return static_cast<size_t>(kMaxUnits) * 4 + static_cast<size_t>(kMaxCtas) * 2 * kPartFloats * 4;
 }
 

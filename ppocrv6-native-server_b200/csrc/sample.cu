@@ -890,7 +890,7 @@ template <int TYPE> cudaError_t sample_type(const SampleArgs &a, cudaStream_t st
     ctas *= 2;
   auto *kernel = sample_row_kernel<TYPE>;
   const int smem = (granules + ctas - 1) / ctas * 16;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost * 16);
+  cudaError_t e = prepare_kernel(reinterpret_cast<const void *>(kernel), kMost * 16);
   if (e != cudaSuccess)
     return e;
   cudaLaunchAttribute attr[2];
