@@ -4,8 +4,10 @@
 // The work is the reading of the cache (D/2 + D/8 bytes per key and as many
 // per value, 160 together at D = 128), so it is split over key tiles, not
 // over heads: the tiles of all (sequence, row group, key head) units are laid
-// end to end and every CTA takes an equal run of them, whatever the lengths
-// (each CTA scans the lengths itself). A unit that several CTAs share is
+// end to end, each unit with kUnitCost tiles' worth of its own costs before
+// them, and every CTA takes an equal run, whatever the lengths (each CTA scans
+// the lengths itself). A run's end that falls near a unit's is moved there,
+// and short units are not split at all. A unit that several CTAs share is
 // joined by the last of them to finish, from fp32 parts (m, l, O) in the
 // workspace, in the order of the CTAs.
 //
@@ -41,7 +43,9 @@ namespace {
 constexpr int kTile = 128;    // keys per stage
 constexpr int kWarps = 4;     // consumers, 32 keys of a tile each
 constexpr int kRowsThreads = 32 * (kWarps + 1);
-constexpr int kMinTiles = 2;  // tiles a CTA takes at least
+constexpr int kUnitCost = 2;  // of a unit (queries, merging, joining), in tiles
+constexpr int kMinQuota = 3;  // of a CTA's run, so counted
+constexpr int kWhole = 4;     // units of fewer tiles are not split
 constexpr int kMaxEntries = 2048; // (sequence, row group) entries per launch
 constexpr int kMaxUnits = 1 << 16; // counters in the workspace
 constexpr int kMaxCtas = 148 * 3;
@@ -131,10 +135,11 @@ __device__ __forceinline__ TileSpan span_of(const RowsArgs &g, const Group &x) {
   return s;
 }
 
-// A position in the sequence of all tiles: entry (sequence, row group), key
-// head, tile of that unit.
+// A unit on the line of all units: entry (sequence, row group), key head, its
+// tiles, and where it starts (kUnitCost places before its first tile).
 struct Cursor {
-  int e, h, cnt, base, j;
+  int e, h, cnt, base;
+  // The unit that holds place t.
   __device__ __forceinline__ void start(const int *prefix, int entries, int kv_heads, int t) {
     int lo = 0, hi = entries; // prefix[lo] <= t < prefix[hi]
     while (hi - lo > 1) {
@@ -145,21 +150,46 @@ struct Cursor {
         hi = mid;
     }
     e = lo;
-    cnt = (prefix[e + 1] - prefix[e]) / kv_heads;
-    h = (t - prefix[e]) / cnt;
-    base = prefix[e] + h * cnt;
-    j = t - base;
+    const int places = (prefix[e + 1] - prefix[e]) / kv_heads;
+    h = (t - prefix[e]) / places;
+    base = prefix[e] + h * places;
+    cnt = places - kUnitCost;
   }
   __device__ __forceinline__ void next_unit(const int *prefix, int kv_heads) {
-    base += cnt;
-    j = 0;
+    base = end();
     if (++h == kv_heads) {
       h = 0;
       do
         ++e;
       while (prefix[e + 1] == prefix[e]);
-      cnt = (prefix[e + 1] - prefix[e]) / kv_heads;
+      cnt = (prefix[e + 1] - prefix[e]) / kv_heads - kUnitCost;
     }
+  }
+  __device__ __forceinline__ int end() const { return base + kUnitCost + cnt; }
+  // The first tile of this unit in a run that starts, or its end in one that
+  // ends, at place t.
+  __device__ __forceinline__ int tile_at(int t) const { return min(max(t - base - kUnitCost, 0), cnt); }
+};
+// How the line is cut into runs.
+struct Cuts {
+  int quota, slack;
+  // Where the cut at place t goes.
+  __device__ __forceinline__ int place(const int *prefix, int entries, int kv_heads, int t) const {
+    const int total = prefix[entries];
+    if (t >= total)
+      return total;
+    Cursor c;
+    c.start(prefix, entries, kv_heads, t);
+    const int j = t - c.base, left = c.end() - t;
+    if (c.cnt < kWhole)
+      return j <= left ? c.base : c.end();
+    return j <= kUnitCost + slack ? c.base : left <= slack ? c.end() : t;
+  }
+  // The CTAs that share a unit: `first` and the parts' number.
+  __device__ __forceinline__ int parts(const Cursor &c, int &first) const {
+    const int lo = (c.base + kUnitCost + slack) / quota + 1, hi = (c.end() - slack - 1) / quota;
+    first = lo - 1;
+    return c.cnt < kWhole || hi < lo ? 1 : hi - lo + 2;
   }
 };
 
@@ -250,13 +280,14 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
   }
   pdl_wait();
 
-  // Tiles before each entry.
+  // Places before each entry.
   {
     const int per = (entries + kRowsThreads - 1) / kRowsThreads;
     const int e0 = tid * per, e1 = min(e0 + per, entries);
     int sum = 0;
     for (int e = e0; e < e1; ++e) {
-      const int n = span_of(g, group_of<kRows>(g, g.b0 + e / g.nrg, g.rg0 + e % g.nrg)).n * g.kv_heads;
+      int n = span_of(g, group_of<kRows>(g, g.b0 + e / g.nrg, g.rg0 + e % g.nrg)).n;
+      n = n ? (n + kUnitCost) * g.kv_heads : 0;
       prefix[e + 1] = n;
       sum += n;
     }
@@ -290,8 +321,11 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
     __syncthreads();
   }
   const int total = prefix[entries];
-  const int quota = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kMinTiles);
-  const int t0 = blockIdx.x * quota, t1 = min(t0 + quota, total);
+  Cuts cuts;
+  cuts.quota = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), kMinQuota);
+  cuts.slack = min(max(cuts.quota / 4, 1), 3);
+  const int t0 = cuts.place(prefix, entries, g.kv_heads, min(static_cast<int>(blockIdx.x) * cuts.quota, total));
+  const int t1 = cuts.place(prefix, entries, g.kv_heads, min(static_cast<int>(blockIdx.x + 1) * cuts.quota, total));
   if (t0 >= t1)
     return;
 
@@ -301,15 +335,15 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
     // ------------------------------------------------------------ producer
     const int page = 1 << g.t.page_shift;
     int fill = 0;
-    for (int t = t0; t < t1;) {
+    for (;;) {
       const int b = g.b0 + cur.e / g.nrg;
       const Group x = group_of<kRows>(g, b, g.rg0 + cur.e % g.nrg);
       const TileSpan span = span_of(g, x);
-      const int end = min(t1, cur.base + cur.cnt);
+      const int end = cur.tile_at(t1);
       bool ok = true;
-      for (; t < end; ++t, ++cur.j, ++fill) {
+      for (int j = cur.tile_at(t0); j < end; ++j, ++fill) {
         const int stage = fill % kStages;
-        const int pos = span.tile(cur.j) * kTile + lane * page;
+        const int pos = span.tile(j) * kTile + lane * page;
         const bool have = lane * page < kTile && pos < x.s.len;
         const long long block =
             have ? static_cast<long long>(kv4_page(g.t, b, pos)) * g.kv_heads + cur.h : 0;
@@ -335,8 +369,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
           *abort = 1;
         break;
       }
-      if (t < t1)
-        cur.next_unit(prefix, g.kv_heads);
+      if (cur.end() >= t1)
+        break;
+      cur.next_unit(prefix, g.kv_heads);
     }
     if (lane == 0 && *abort) {
       // No copy may land after the CTA is gone.
@@ -383,7 +418,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
   }
   bool ok = true;
   int fill = 0;
-  for (int t = t0; t < t1;) {
+  for (;;) {
     const int b = g.b0 + cur.e / g.nrg;
     const Group x = group_of<kRows>(g, b, g.rg0 + cur.e % g.nrg);
     const TileSpan span = span_of(g, x);
@@ -473,9 +508,9 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
           o[d][nt][i] = 0.f;
     }
 
-    const int end = min(t1, cur.base + cur.cnt);
-    const bool from_start = t == cur.base, to_end = end == cur.base + cur.cnt;
-    for (; t < end; ++t, ++cur.j, ++fill) {
+    const int begin = cur.tile_at(t0), end = cur.tile_at(t1);
+    const bool from_start = begin == 0, to_end = end == cur.cnt;
+    for (int j = begin; j < end; ++j, ++fill) {
       const int stage = fill % kStages;
       if (!mbar_wait(full + stage, (fill / kStages) & 1, abort)) {
         // Lost arrival: everybody stops waiting, the CTA runs out and the
@@ -483,7 +518,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
         ok = false;
         *abort = 1;
       }
-      const int key0 = span.tile(cur.j) * kTile + warp * 32;
+      const int key0 = span.tile(j) * kTile + warp * 32;
       const uint32_t st = stage * L::kStageBytes;
       // Whether every row sees all of this warp's keys.
       const bool clear = key0 + 31 <= x.pos_lo &&
@@ -759,7 +794,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
     }
     if (!whole) {
       // ---- the last CTA to finish joins the unit's parts
-      const int first = cur.base / quota, parts = (cur.base + cur.cnt - 1) / quota - first + 1;
+      int first;
+      const int parts = cuts.parts(cur, first);
       consumer_barrier();
       if (tid == 0) {
         int *c = g.counters + cur.e * g.kv_heads + cur.h;
@@ -773,10 +809,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
       consumer_barrier();
       if (*is_last) {
         auto part_of = [&](int i) {
-          // The unit's first CTA went out on it unless the unit starts there.
-          const int cta = first + i;
-          const bool began = cur.base >= cta * quota;
-          return g.parts + static_cast<long long>(cta * 2 + (began ? 1 : 0)) * kPartFloats;
+          // The unit's first CTA went out on it, the others came in.
+          return g.parts + static_cast<long long>((first + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats;
         };
         // Largest maximum of each row, by 32 kWarps / kRows threads each.
         float best = -INFINITY;
@@ -807,9 +841,10 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
         }
       }
     }
+    if (cur.end() >= t1)
+      break;
     consumer_barrier();
-    if (t < t1)
-      cur.next_unit(prefix, g.kv_heads);
+    cur.next_unit(prefix, g.kv_heads);
   }
   if (!ok && lane == 0)
     kv4_fault(g.t, kErrRowsWait);
@@ -863,7 +898,11 @@ cudaError_t kv4_attend_rows(const Kv4Cache &c, const Kv4Tokens &t, const Kv4Atte
   const long long rows = static_cast<long long>(t.max_new) * g.group;
   const int nt = rows <= 8 ? 1 : 2;
   const long long groups = (rows + 8 * nt - 1) / (8 * nt);
-  const long long most = std::min<long long>(kMaxEntries, kMaxUnits / c.kv_heads);
+  // Places on the line are counted in 31 bits.
+  const long long room = (static_cast<long long>(t.width) * c.page_size + kTile - 1) / kTile + kUnitCost;
+  const long long most = std::max<long long>(
+      1, std::min({static_cast<long long>(kMaxEntries), static_cast<long long>(kMaxUnits / c.kv_heads),
+                   ((1ll << 31) - 1) / (c.kv_heads * room)}));
   const int per_rg = static_cast<int>(std::min<long long>(groups, most));
   const int per_b = static_cast<int>(std::max<long long>(1, most / per_rg));
   for (int b = 0; b < t.batch; b += per_b)
