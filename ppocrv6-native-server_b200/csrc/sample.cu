@@ -13,8 +13,9 @@
 //  1. the maximum, the masses and their sum;
 //  2. a bound below which the prefix cannot end: for top-k the smallest
 //     logit L such that every warp has its share of k logits at or above it;
-//     for top-p the mass (1 - p) sum / V (all that is lighter cannot make up
-//     1 - p together), or min-p where that is more;
+//     for top-p the largest of four levels whose lighter logits make up less
+//     than 1 - p together (summed in step 1), at least (1 - p) sum / V, or
+//     min-p where that is more;
 //  3. a histogram of counts and masses of what passes the bound, over 512
 //     steps of max - x: its running sums say in which step the prefix ends;
 //  4. the logits of that step, sorted and summed in order (every CTA does
@@ -30,6 +31,7 @@
 #include "ptx.cuh"
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 #include <cuda_bf16.h>
 
 namespace pb2 {
@@ -58,6 +60,17 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 __device__ __forceinline__ float share_of(float x, float top, float t) {
   return x == top ? 1.f : expf(-__fdiv_rn(__fsub_rn(top, x), t));
+}
+// d / t correctly rounded without a branch, for r = 1 / t correctly rounded
+// and neither result nor remainder beyond the normal numbers: two steps of
+// q + (d - q t) r with fused multiply-adds (P. Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", IBM J. Res.
+// Dev. 34, 1990). Infinite d gives NaN, tiny quotients may be off in their
+// last bit; as exp(-q), that is no mass and 1.
+__device__ __forceinline__ float quotient(float d, float t, float r) {
+  float q = __fmul_rn(d, r);
+  q = __fmaf_rn(__fmaf_rn(-q, t, d), r, q);
+  return __fmaf_rn(__fmaf_rn(-q, t, d), r, q);
 }
 __device__ __forceinline__ u64 mass_of(float e) { return __float2ull_rz(e * 4294967296.f); }
 // floor(whole * share / 2^24) for share <= 2^24, whole < 2^57.
@@ -275,8 +288,14 @@ constexpr int kCap = 1024;    // logits that are sorted at most
 constexpr int kMostCtas = 8;
 constexpr float kReach = 22.2f; // exp(-22.2) < 2^-32: no mass past it
 
+constexpr int kLevels = 4;
+__device__ __forceinline__ float level_of(int l) { // 1e-2, 1e-3, 1e-4, 1e-5 of the most probable
+  return l == 0 ? 1e-2f : l == 1 ? 1e-3f : l == 2 ? 1e-4f : 1e-5f;
+}
+
 struct Part { // one CTA's sums
-  u64 all, likely; // mass; mass at or above min-p
+  u64 all, likely;      // mass; mass at or above min-p
+  float below[kLevels]; // about: what is lighter than each level
   int likely_n;
   uint32_t bound;  // smallest key that passes the top-k bound
 };
@@ -290,6 +309,8 @@ struct ClusterShared {
     } bins;
     Digits digits;
   };
+  u64 bin_mass[kBins]; // of the whole row
+  int bin_count[kBins];
   u64 keys[2][kCap]; // of the step where top-k and top-p end
   int taken[2];
   Ends ends[kMostCtas], warp_ends[32];
@@ -437,7 +458,7 @@ __device__ __noinline__ Prefix resolve(ClusterShared &sh, u64 *keys, int n, int 
 constexpr int kRowThreads = 512;
 
 template <int TYPE>
-__global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ uint4 granules[]; // this CTA's run of the row
   __shared__ ClusterShared sh;
   constexpr int kSize = TYPE == LOGIT_F32 ? 4 : 2;
@@ -505,28 +526,50 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
   float top = -INFINITY, low = INFINITY;
   {
     constexpr uint32_t kNegInf = TYPE == LOGIT_F32 ? 0xFF800000u : TYPE == LOGIT_BF16 ? 0xFF80u : 0xFC00u;
-#pragma unroll 4
-    for (int g = g0 + lane; g < g1; g += 32) {
-      uint4 w = __ldg(base + cta0 + g);
-      uint32_t in[4] = {w.x, w.y, w.z, w.w};
-      const bool edge = index_of(g, 0) < 0 || index_of(g, kVec) > V;
+    constexpr int kBatch = 8; // loads on their way at once
+    for (int gb = g0 + lane; gb < g1; gb += 32 * kBatch) {
+      uint4 ws[kBatch];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        const float v = at(w, j);
-        bool bad = !(v == v);
-        if (edge)
-          bad = bad || index_of(g, j) < 0 || index_of(g, j) >= V;
-        if (bad) {
-          if constexpr (TYPE == LOGIT_F32)
-            in[j] = kNegInf;
-          else
-            in[j / 2] = j & 1 ? (in[j / 2] & 0xFFFFu) | kNegInf << 16 : (in[j / 2] & 0xFFFF0000u) | kNegInf;
-        } else {
-          top = fmaxf(top, v);
-          low = v > -INFINITY ? fminf(low, v) : low;
+      for (int q = 0; q < kBatch; ++q)
+        if (gb + 32 * q < g1)
+          ws[q] = __ldg(base + cta0 + gb + 32 * q);
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) {
+        const int g = gb + 32 * q;
+        if (g >= g1)
+          break;
+        uint32_t in[4] = {ws[q].x, ws[q].y, ws[q].z, ws[q].w};
+        const bool edge = index_of(g, 0) < 0 || index_of(g, kVec) > V;
+        float high = -INFINITY, least = INFINITY;
+        bool odd = edge;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const float v = at(ws[q], j);
+          high = fmaxf(high, v); // passes over NaN
+          least = fminf(least, v);
+          odd = odd || !(v > -INFINITY);
         }
+        if (odd) { // NaN, -inf, or the row's first or last granule
+          high = -INFINITY;
+          least = INFINITY;
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            const float v = at(ws[q], j);
+            if (!(v == v) || index_of(g, j) < 0 || index_of(g, j) >= V) {
+              if constexpr (TYPE == LOGIT_F32)
+                in[j] = kNegInf;
+              else
+                in[j / 2] = j & 1 ? (in[j / 2] & 0xFFFFu) | kNegInf << 16 : (in[j / 2] & 0xFFFF0000u) | kNegInf;
+            } else {
+              high = fmaxf(high, v);
+              least = v > -INFINITY ? fminf(least, v) : least;
+            }
+          }
+        }
+        top = fmaxf(top, high);
+        low = fminf(low, least);
+        granules[g] = make_uint4(in[0], in[1], in[2], in[3]);
       }
-      granules[g] = make_uint4(in[0], in[1], in[2], in[3]);
     }
   }
   __syncwarp();
@@ -592,7 +635,8 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
   Part own{};
   {
     unsigned ones = 0; // masses of 2^32, one short in 32 bits
-    auto add = [&](auto divide, auto bounded) {
+    const float inverse = __frcp_rn(t);
+    auto add = [&](auto exact, auto bounded, auto levels) {
 #pragma unroll 1
       for (int g = g0 + lane; g < g1; g += 32) {
         const uint4 w = granules[g];
@@ -600,26 +644,32 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
         for (int j = 0; j < kVec; ++j) {
           const float v = at(w, j);
           const float d = __fsub_rn(top, v);
-          const float e = v == top ? 1.f : expf(-(divide ? __fdiv_rn(d, t) : d));
+          const float e = v == top ? 1.f : expf(-(exact.value ? __fdiv_rn(d, t) : quotient(d, t, inverse)));
           const uint32_t m = __float2uint_rz(e * 4294967296.f);
           own.all += m;
           ones += e == 1.f;
-          if (bounded && e >= mp) {
+          if constexpr (levels.value) {
+#pragma unroll
+            for (int l = 0; l < kLevels; ++l)
+              own.below[l] += e < level_of(l) ? e : 0.f;
+          }
+          if (bounded.value && e >= mp) {
             own.likely += m + static_cast<u64>(e == 1.f);
             ++own.likely_n;
           }
         }
       }
     };
-    struct No { __device__ constexpr operator bool() const { return false; } };
-    struct Yes { __device__ constexpr operator bool() const { return true; } };
-    if (mp > 0.f) {
-      add(Yes{}, Yes{});
-    } else if (t == 1.f) {
-      add(No{}, No{});
-    } else {
-      add(Yes{}, No{});
-    }
+    using No = std::false_type;
+    using Yes = std::true_type;
+    if (!(t > 1e-30f && t < 1e30f))
+      add(Yes{}, Yes{}, Yes{});
+    else if (mp > 0.f)
+      add(No{}, Yes{}, Yes{});
+    else if (by_p && !by_k)
+      add(No{}, No{}, Yes{});
+    else
+      add(No{}, No{}, No{});
     own.all += ones;
   }
   if (mp > 0.f) {
@@ -627,14 +677,25 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
     own.likely = warp_sum(own.likely);
   }
   own.all = warp_sum(own.all);
+  auto sum_below = [&](Part &x) {
+    if (by_p && !by_k)
+#pragma unroll
+      for (int l = 0; l < kLevels; ++l)
+#pragma unroll
+        for (int o = 16; o; o /= 2)
+          x.below[l] += __shfl_xor_sync(~0u, x.below[l], o);
+  };
+  sum_below(own);
   own.bound = bound;
   if (lane == 0)
     sh.warp_part[warp] = own;
   __syncthreads();
   if (warp == 0) {
-    Part z{0, 0, 0, 0xFFFFFFFFu};
+    Part z{0, 0, {}, 0, 0xFFFFFFFFu};
     if (lane < kWarps)
       z = sh.warp_part[lane];
+    sum_below(z);
+    own = z;
     own.all = warp_sum(z.all);
     own.likely = warp_sum(z.likely);
     own.likely_n = __reduce_add_sync(~0u, z.likely_n);
@@ -650,6 +711,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
     sum.likely += y.likely;
     sum.likely_n += y.likely_n;
     sum.bound = min(sum.bound, y.bound);
+#pragma unroll
+    for (int l = 0; l < kLevels; ++l)
+      sum.below[l] += y.below[l];
   }
 
   // Calls body(x, index) for this warp's logits that pass `test`, each lane
@@ -684,10 +748,13 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
   } else if (by_k || by_p) {
     float least = by_k ? value_of(max(sum.bound, key_of(-INFINITY))) : -INFINITY;
     if (!by_k) {
-      // Shares below this make up less than 1 - p, with a quarter to spare
-      // for the masses' rounding down and this bound's own.
+      // What is lighter than this makes up less than 1 - p, with a quarter to
+      // spare for roundings.
       const float rest = 0.75f * (1.f - static_cast<float>(p24) * 0x1p-24f) * (__ull2float_rn(sum.all) * 0x1p-32f);
-      const float share = fmaxf(rest / static_cast<float>(V), mp * 0.99f);
+      float share = fmaxf(rest / static_cast<float>(V), mp * 0.99f);
+#pragma unroll
+      for (int l = 0; l < kLevels; ++l)
+        share = sum.below[l] <= rest ? fmaxf(share, 0.99f * level_of(l)) : share;
       if (share > 0x1p-31f && share <= 1.f)
         least = top + t * logf(share) * 1.0001f - 1e-6f * fabsf(top);
     }
@@ -704,33 +771,46 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
                const int b = bin_of(v);
                const u64 w = mass_of(share_of(v, top, t));
                atomicAdd(&sh.bins.count[b], 1u);
-               // 16 bits at a time: at most 2^15 logits of a CTA a step carry
-               // mass (the launcher's bound on a run), no carry is lost.
+               // 16 bits at a time: fewer than 2^16 logits a CTA, no carry
+               // is lost.
                if (w) {
                  atomicAdd(&sh.bins.lo[b], static_cast<unsigned>(w) & 0xFFFFu);
                  atomicAdd(&sh.bins.hi[b], static_cast<unsigned>(w >> 16));
                }
              });
     cluster_sync();
-    // Every CTA sums and scans all of it: two neighbouring steps a thread.
+    // Each CTA sums a share of the steps over the CTAs and gives it to all.
+    {
+      const int per = kBins / ctas; // 1, 2, 4 or 8 CTAs
+      for (int i = tid; i < per; i += kRowThreads) {
+        const int b = rank * per + i;
+        u64 m = 0;
+        int n = 0;
+        for (int c = 0; c < ctas; ++c) {
+          const auto *h = remote(&sh.bins, c);
+          m += h->lo[b] + (static_cast<u64>(h->hi[b]) << 16);
+          n += static_cast<int>(h->count[b]);
+        }
+        for (int c = 0; c < ctas; ++c) {
+          *remote(&sh.bin_mass[b], c) = m;
+          *remote(&sh.bin_count[b], c) = n;
+        }
+      }
+    }
+    cluster_sync(); // and the digit search may use the bins' space
+    // Every CTA scans them: two neighbouring steps a thread.
     u64 mass[2] = {0, 0};
     int count[2] = {0, 0};
     if (2 * tid < kBins) {
-      for (int c = 0; c < ctas; ++c) {
-        const auto *h = remote(&sh.bins, c);
-        const uint2 n2 = *reinterpret_cast<const uint2 *>(h->count + 2 * tid);
-        const uint2 l2 = *reinterpret_cast<const uint2 *>(h->lo + 2 * tid);
-        const uint2 h2 = *reinterpret_cast<const uint2 *>(h->hi + 2 * tid);
-        count[0] += static_cast<int>(n2.x);
-        count[1] += static_cast<int>(n2.y);
-        mass[0] += l2.x + (static_cast<u64>(h2.x) << 16);
-        mass[1] += l2.y + (static_cast<u64>(h2.y) << 16);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        mass[q] = sh.bin_mass[2 * tid + q];
+        count[q] = sh.bin_count[2 * tid + q];
       }
     }
     u64 m0 = mass[0] + mass[1], m_total;
     int n0 = count[0] + count[1], n_total;
     block_scan(m0, n0, sh, m_total, n_total);
-    bool drained = false; // whether every CTA has read the bins
     auto end_in = [&](bool by_mass, u64 want) {
       if (by_mass && m_total < want) // min-p ends it before p does
         return Prefix{0, V, INT_MAX, sum.all};
@@ -755,9 +835,6 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
       const int b = sh.edge_bin, n_in = sh.edge_count, n_before = sh.edge_before;
       const u64 m_before = sh.edge_mass;
       if (n_in > kCap) { // ---- 4. too many near each other
-        if (!drained)
-          cluster_sync(); // the digit search takes the bins' place
-        drained = true;
         return select<TYPE>(row, V, top, t, by_mass, want, sh.digits);
       }
       // Every CTA gets all logits of the step.
@@ -769,7 +846,6 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
                    remote(&sh.keys[slot][0], c)[atomicAdd(remote(&sh.taken[slot], c), 1)] = key;
                });
       cluster_sync();
-      drained = true;
       return resolve(sh, sh.keys[slot], n_in, n_before, m_before, by_mass, want, top, t);
     };
     if (by_k)
@@ -793,7 +869,12 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
   const bool edge_passes = p.key && share_of(edge, top, t) >= mp;
   u64 mine = 0;
   int ties = 0;
-  each_hit([&](float v) { return v >= edge && v > -INFINITY; },
+  // Nothing below this has a mass that stays.
+  float from = edge;
+  if (p.key == 0 && mp > 0.f)
+    from = top + t * logf(mp * 0.99f) * 1.0001f - 1e-6f * fabsf(top);
+  from = from == from ? fminf(from, top) : -INFINITY;
+  each_hit([&](float v) { return v >= from && v > -INFINITY; },
            [&](float v, int) {
              mine += sure(v);
              ties += edge_passes && v == edge;
@@ -875,16 +956,16 @@ __global__ void __launch_bounds__(kRowThreads, 3) sample_row_kernel(const __grid
 
 template <int TYPE> cudaError_t sample_type(const SampleArgs &a, cudaStream_t stream) {
   constexpr int kVec = TYPE == LOGIT_F32 ? 4 : 8;
-  // Granules of 16 bytes that a row may touch; a CTA's run has at most 2^15
-  // logits (the histogram's sums).
+  // Granules of 16 bytes that a row may touch. A CTA's run has at most 60000
+  // logits (the histogram's sums of 16-bit halves) in 192 KB.
   const int granules = a.vocab / kVec + 2;
-  constexpr int kMost = (1 << 15) / kVec;
+  constexpr int kMost = TYPE == LOGIT_F32 ? 12288 : 7424; // granules
   if (granules > kMostCtas * kMost)
     return launch_pdl(sample_long_kernel<TYPE>, a.rows, kThreads, 0, stream, a);
-  // CTAs per row: while all rows fit the GPU at once (three an SM) and a CTA
+  // CTAs per row: while all rows fit the GPU at once (two an SM) and a CTA
   // has 2048 logits or more, spread them; then as many as a row needs.
   int ctas = 1;
-  while (ctas < kMostCtas && a.rows * 2ll * ctas <= 3ll * sm_count() && granules > ctas * 4096 / kVec)
+  while (ctas < kMostCtas && a.rows * 2ll * ctas <= 2ll * sm_count() && granules > ctas * 4096 / kVec)
     ctas *= 2;
   while (ctas < kMostCtas && granules > ctas * kMost)
     ctas *= 2;
