@@ -1,0 +1,197 @@
+"""A small autoregressive text decoder over the recognizer's hidden states:
+the operators of `ppocr_b200.decode` together with the framework's GEMM and
+LayerNorm, as a serving program would run them.
+
+    python -m ppocr_b200.textgen [--lines N] [--tokens N]
+
+reads N random line images with the compiled recognizer, takes each line's
+hidden states as the prompt of a randomly initialised decoder and generates
+tokens: prompts and single tokens go through the 4-bit cache, and every token
+is drawn on the device.
+"""
+
+from __future__ import annotations
+
+import argparse
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from . import capi, decode
+
+BIAS, SWISH = 0, 5  # activation codes of ppocr_b200_gemm_epilogue
+
+
+@dataclass(frozen=True)
+class DecoderShape:
+    inputs: int            # channels of the prompt's hidden states
+    vocab: int
+    dim: int = 512
+    layers: int = 2
+    heads: int = 8
+    kv_heads: int = 4
+    head_dim: int = 64
+    mlp: int = 1024
+    window: int = 0        # 0: every earlier position is seen
+    sinks: int = 0
+
+
+class DecoderWeights:
+    """FP16 device weights, [out][in]; rows of the vocabulary head are padded
+    to a multiple of 8 with zeros."""
+
+    def __init__(self, shape: DecoderShape, device: torch.device, positions: int, seed: int = 0):
+        g = torch.Generator(device="cpu").manual_seed(seed)
+
+        def linear(out: int, inp: int) -> torch.Tensor:
+            return (torch.randn(out, inp, generator=g) * inp ** -0.5).half().to(device)
+
+        s = shape
+        self.inp = linear(s.dim, s.inputs)
+        self.tokens = (torch.randn(s.vocab, s.dim, generator=g) * 0.5).half().to(device)
+        self.positions = (torch.randn(positions, s.dim, generator=g) * 0.1).half().to(device)
+        self.qkv = [linear((s.heads + 2 * s.kv_heads) * s.head_dim, s.dim) for _ in range(s.layers)]
+        self.out = [linear(s.dim, s.heads * s.head_dim) for _ in range(s.layers)]
+        self.up = [linear(s.mlp, s.dim) for _ in range(s.layers)]
+        self.down = [linear(s.dim, s.mlp) for _ in range(s.layers)]
+        self.norms = [torch.ones(s.dim, dtype=torch.float16, device=device) for _ in range(2 * s.layers + 1)]
+        self.zero = torch.zeros(s.dim, dtype=torch.float16, device=device)
+        self.head = torch.zeros((s.vocab + 7) // 8 * 8, s.dim, dtype=torch.float16, device=device)
+        self.head[: s.vocab] = linear(s.vocab, s.dim)
+
+
+class TextDecoder:
+    """Decoder with a 4-bit cache for up to `batch` sequences of up to
+    `max_len` tokens (prompt and answer)."""
+
+    def __init__(self, shape: DecoderShape, weights: DecoderWeights, batch: int, max_len: int,
+                 device: torch.device | str = "cuda:0", page_size: int = 32):
+        self.shape, self.weights = shape, weights
+        self.lib = capi.load()
+        self.batch = batch
+        width = -(-max_len // page_size)
+        self.max_len = width * page_size
+        self.caches = [decode.KvCache4(batch * width, page_size, shape.kv_heads, shape.head_dim, device=device)
+                       for _ in range(shape.layers)]
+        self.device = self.caches[0].device
+        # Every sequence owns `width` pages; the tables of all layers agree.
+        self.table = torch.arange(batch * width, dtype=torch.int32, device=self.device).view(batch, width)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=self.device)
+
+    def _stream(self) -> int:
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _gemm(self, x: torch.Tensor, w: torch.Tensor, act: int = BIAS, residual: torch.Tensor | None = None):
+        y = torch.empty(x.shape[0], w.shape[0], dtype=torch.float16, device=self.device)
+        capi.check(self.lib.ppocr_b200_gemm_epilogue(
+            x.data_ptr(), w.data_ptr(), None, residual.data_ptr() if residual is not None else None, y.data_ptr(),
+            x.shape[0], x.shape[1], w.shape[0], act, ctypes.c_void_p(self._stream())))
+        return y
+
+    def _norm(self, x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+        y = torch.empty_like(x)
+        capi.check(self.lib.ppocr_b200_layernorm(
+            x.data_ptr(), scale.data_ptr(), self.weights.zero.data_ptr(), y.data_ptr(), x.shape[0], x.shape[1], 1e-5,
+            ctypes.c_void_p(self._stream())))
+        return y
+
+    def _layers(self, x: torch.Tensor, starts: torch.Tensor | None, max_new: int | None) -> torch.Tensor:
+        """The decoder's blocks over packed rows x of each sequence's last tokens."""
+        s, w = self.shape, self.weights
+        kv = s.kv_heads * s.head_dim
+        for n in range(s.layers):
+            qkv = self._gemm(self._norm(x, w.norms[2 * n]), w.qkv[n])
+            q, k, v = qkv.split([s.heads * s.head_dim, kv, kv], dim=1)
+            cache = self.caches[n]
+            cache.append(k.unflatten(1, (s.kv_heads, -1)), v.unflatten(1, (s.kv_heads, -1)), self.table, self.lengths,
+                         starts=starts, max_new=max_new)
+            o = cache.attention(q.unflatten(1, (s.heads, -1)), self.table, self.lengths, starts=starts,
+                                max_new=max_new, window=s.window, sinks=s.sinks)
+            x = self._gemm(o.flatten(1), w.out[n], residual=x)
+            x = self._gemm(self._gemm(self._norm(x, w.norms[2 * n + 1]), w.up[n], SWISH), w.down[n], residual=x)
+        return x
+
+    def _logits(self, x: torch.Tensor) -> torch.Tensor:
+        return self._gemm(self._norm(x, self.weights.norms[-1]), self.weights.head)[:, : self.shape.vocab]
+
+    def prompt(self, hidden: torch.Tensor, lengths: list[int]) -> torch.Tensor:
+        """Starts every sequence: hidden [sum(lengths), inputs] FP16, packed;
+        returns the logits [batch, vocab] after each prompt's last token."""
+        if len(lengths) != self.batch or min(lengths) < 1 or max(lengths) > self.max_len:
+            raise ValueError(f"{self.batch} prompts of 1 to {self.max_len} tokens")
+        if hidden.shape != (sum(lengths), self.shape.inputs):
+            raise ValueError(f"hidden must be [{sum(lengths)}, {self.shape.inputs}]")
+        new = torch.tensor(lengths, dtype=torch.int32)
+        starts = torch.zeros(self.batch + 1, dtype=torch.int32)
+        starts[1:] = new.cumsum(0)
+        starts = starts.to(self.device)
+        self.lengths.copy_(new)
+        pos = torch.cat([torch.arange(n) for n in lengths]).to(self.device)
+        x = self._gemm(hidden.contiguous(), self.weights.inp, residual=self.weights.positions[pos])
+        x = self._layers(x, starts, max(lengths))
+        return self._logits(x[starts[1:].long() - 1])
+
+    def step(self, ids: torch.Tensor) -> torch.Tensor:
+        """One more token per sequence (ids [batch]): the next logits."""
+        pos = self.lengths.long()
+        self.lengths += 1
+        ids = ids.long().clamp(min=0)
+        x = self.weights.tokens[ids] + self.weights.positions[pos]
+        return self._logits(self._layers(x, None, None))
+
+    def generate(self, hidden: torch.Tensor, lengths: list[int], tokens: int, uniform: torch.Tensor,
+                 temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+                 top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None):
+        """`tokens` tokens per sequence with the random numbers uniform
+        [tokens, batch]: (ids [tokens, batch], probabilities [tokens, batch]).
+        Nothing waits for the GPU between steps."""
+        if max(lengths) + tokens - 1 > self.max_len:
+            raise ValueError(f"prompt and answer exceed {self.max_len} tokens")
+        logits = self.prompt(hidden, lengths)
+        ids, probs = [], []
+        for n in range(tokens):
+            i, p, _ = decode.sample(logits, uniform[n], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            ids.append(i)
+            probs.append(p)
+            if n + 1 < tokens:
+                logits = self.step(i)
+        return torch.stack(ids), torch.stack(probs)
+
+
+def main() -> None:
+    from . import pipeline
+
+    ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
+    ap.add_argument("--lines", type=int, default=2)
+    ap.add_argument("--tokens", type=int, default=16)
+    a = ap.parse_args()
+    rec = pipeline.LineRecognizer("rec_b2" if a.lines <= 2 else "rec_b64")
+    try:
+        if not 1 <= a.lines <= rec.batch:
+            ap.error(f"--lines must be 1 to {rec.batch}")
+        g = torch.Generator(device=rec.device).manual_seed(7)
+        x = torch.rand(a.lines, *rec.model.input_shape[2:], 3, device=rec.device, generator=g).half() * 2 - 1
+        with torch.cuda.stream(rec.stream):
+            rec.enqueue(x)
+            shape = DecoderShape(inputs=rec.H, vocab=rec.vocab)
+            weights = DecoderWeights(shape, rec.device, positions=rec.T + a.tokens)
+            decoder = TextDecoder(shape, weights, a.lines, rec.T + a.tokens, device=rec.device)
+            lengths = [rec.T] * a.lines
+            full = lambda v: torch.full((a.lines,), v, device=rec.device)  # noqa: E731
+            ids, probs = decoder.generate(
+                rec.hidden[: a.lines].reshape(-1, rec.H), lengths, a.tokens,
+                torch.rand(a.tokens, a.lines, device=rec.device, generator=g), temperature=full(0.8),
+                top_k=full(50).int(), top_p=full(0.95))
+        torch.cuda.synchronize(rec.device)
+        code = capi.load().ppocr_b200_device_error()
+        if code:
+            raise SystemExit(f"device error {code}")
+        for n in range(a.lines):
+            print(f"line {n}: ids {ids[:, n].tolist()}  mean probability {probs[:, n].mean().item():.4f}")
+    finally:
+        rec.close()
+
+
+if __name__ == "__main__":
+    main()
