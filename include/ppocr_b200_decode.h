@@ -56,8 +56,8 @@ size_t ppocr_b200_kv4_block_bytes(int page_size, int head_dim);
 // [tokens][kv_heads][head_dim] of the cache's type with rows k_stride and
 // v_stride elements apart (multiples of 8; 16-byte aligned), so slices of a
 // fused projection need no copy. Per group of 32 channels: minimum = min x,
-// scale = round16((max x - min x) / 15), code = clamp(rint((x - minimum) *
-// (1 / scale)), 0, 15), computed in fp32. NaN is stored as 0; values beyond
+// scale = round16((max x - min x) * (1 / 15)), code = clamp(rint((x -
+// minimum) * (1 / scale)), 0, 15), every step rounded to fp32 (1 / 15 too). NaN is stored as 0; values beyond
 // +-65000 (fp16) or +-2^126 (bf16) saturate there.
 int ppocr_b200_kv4_append(const PpocrKv4Cache *cache, const void *k,
                           long long k_stride, const void *v,

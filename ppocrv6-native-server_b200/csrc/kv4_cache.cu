@@ -4,8 +4,7 @@
 // each) and 1.25 go out, or the other way round; next to that the append
 // kernel is close to being bound by its instructions (about nine a value).
 //  * append: a thread owns a group of 32 channels: four 16-byte loads, packed
-//    16-bit minimum and maximum, one division by 15 and one reciprocal per
-//    group, a 16-byte store of codes and a 4-byte one of (scale, minimum).
+//    16-bit minimum and maximum, one reciprocal per group, a 16-byte store of codes and a 4-byte one of (scale, minimum).
 //    Values that are not finite or beyond the limit are looked for in the bit
 //    patterns and put right on a path of their own.
 //  * read: a thread owns eight channels of a key and of its value, so that
@@ -128,7 +127,7 @@ template <bool BF16> __device__ __forceinline__ uint4 quantise(uint4 (&in)[4], u
     mx = max2<BF16>(mx, w[i]);
   }
   const float lo = fminf(kv4_lo<BF16>(mn), kv4_hi<BF16>(mn)), hi = fmaxf(kv4_lo<BF16>(mx), kv4_hi<BF16>(mx));
-  params = kv4_pack<BF16>(__fdiv_rn(__fsub_rn(hi, lo), 15.f), lo);
+  params = kv4_pack<BF16>(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f), lo);
   const float scale = kv4_lo<BF16>(params);
   const float inv = scale > 1e-30f ? __frcp_rn(scale) : 0.f;
   uint32_t codes[4];

@@ -159,6 +159,32 @@ def test_append_unusual_values(native, cuda, dtype):
     assert torch.equal(rk.cpu(), want.to(dtype))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_append_scales_on_rounding_boundaries(native, cuda, dtype):
+    """Groups whose range is 15 times a midpoint of the 16-bit type: the scale
+    is what the fp32 product with 1/15 rounds to, not the quotient."""
+    digits = 11 if dtype == F16 else 8
+    steps = torch.arange(2 ** (digits - 1), 2 ** digits).double() + 0.5  # midpoints
+    high = 15 * steps * 2.0 ** -digits
+    rows = torch.zeros(len(steps), 1, 32)
+    # The range, split over the ends so that both are representable.
+    top = high.to(dtype)
+    rest = (high - top.double()).to(dtype)
+    keep = (top.double() + rest.double() == high)
+    rows[:, 0, 0], rows[:, 0, 1] = top.float(), -rest.float()
+    rows[:, 0, 2:] = (torch.rand(len(steps), 30, generator=gen(50)) * 0.9 + 0.05) * top.float()[:, None]
+    x = rows[keep & (rest.double() >= 0)].to(dtype)
+    assert len(x) >= 16
+    s = Scene([len(x)], [len(x)], 1, 32, 64, dtype, stale="random")
+    s.k, s.v = [x], [x.flip(0)]
+    cache = s.cache()
+    table, lens = s.places()
+    cache.append(x.cuda(), s.v[0].cuda(), table, lens)
+    assert fault(native) == 0
+    s.fill([len(x)])
+    assert torch.equal(cache.pool.cpu(), s.pool)
+
+
 def test_cache_error_of_quantisation(native, cuda):
     """What reads back is within half a step (plus the scale's and the
     output's own rounding) of what was written."""
