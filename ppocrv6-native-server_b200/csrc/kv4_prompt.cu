@@ -186,8 +186,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
   const uint32_t sbase = smem_u32(smem);
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kOffBars);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7;
-  uint64_t *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 13, *drain = bars + 15;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16);
+  uint64_t *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 15, *drain = bars + 17; // p_full: block, half
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 18);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
       mbar_init(k_empty + i, 1);
       mbar_init(v_empty + i, 1);
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 128);
+      mbar_init(p_full + 2 * i, 128);
+      mbar_init(p_full + 2 * i + 1, 128);
       mbar_init(o_full + i, 1);
     }
     mbar_init(drain, 1);
@@ -392,11 +393,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             }
           }
           tmem_st16(t_s + 16 * c, p);
+          if (c & 1) { // the product starts on the first 64 keys
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(p_full + 2 * block + c / 2);
+          }
         }
         l += (sum.x + sum2.x) + (sum.y + sum2.y);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(p_full + block);
       }
       if (ok) {
         ok = mbar_wait(o_full + block, 0, abort);
@@ -622,9 +625,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         }
         umma_commit(s_full + block);
       };
-      auto values = [&](int block, int st, int j) {
+      auto values = [&](int block, int half, int st, int j) {
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
+        for (int k = half * kTile / 32; k < (half + 1) * kTile / 32; ++k)
           umma_ts(tmem + 256 + block * 128, tmem + block * 128 + k * 8,
                   sdesc_mn_sw128(sbase + L::kOffV + st * L::kOperand + k * 2048), idesc_o, j != 0 || k != 0);
       };
@@ -641,11 +644,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         const bool more = j + 1 < tiles;
         ok = mbar_wait(v_full + st, (j / 2) & 1, abort) && (!more || mbar_wait(k_full + next, ((j + 1) / 2) & 1, abort));
         for (int block = 0; ok && block < (two ? 2 : 1); ++block) {
-          ok = mbar_wait(p_full + block, j & 1, abort);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            ok = mbar_wait(p_full + 2 * block + half, j & 1, abort);
+            if (!ok)
+              break;
+            tc_fence_after();
+            values(block, half, st, j);
+          }
           if (!ok)
             break;
-          tc_fence_after();
-          values(block, st, j);
           if (more)
             scores(block, next);
           else
