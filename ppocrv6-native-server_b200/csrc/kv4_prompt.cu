@@ -5,8 +5,11 @@
 // head of the group) pairs, so the heads that share a key head share its
 // restored keys and values. It walks the 128-key tiles that its rows see:
 //  * seven warps restore the tile's keys and values from the cache's pages
-//    (two codes a byte, scale * c + minimum rounded once to the cache's
-//    16-bit type) into shared memory, as rows of a token, 128-byte swizzled;
+//    (two codes a byte, scale * c + minimum rounded once to 16 bits: the
+//    cache's type, but a bf16 cache's values to fp16, divided by a power of two
+//    that follows the largest parameters met, which keeps three bits more and
+//    the sums within fp32) into shared memory, as rows of a token, 128-byte
+//    swizzled;
 //    the next tile's codes are in registers by then. Channels lie in the order 0 4 1 5 2 6 3 7 of every eight, as the
 //    codes' masks give them: queries are reordered alike, the output back;
 //  * one thread issues S = Q K^T for two blocks of 128 rows (K is K-major)
@@ -17,7 +20,8 @@
 //    load's latency is several hundred cycles while products run) and stay in
 //    registers, which the restoring warps give up for that. The running maximum is only raised when a score
 //    passes it by more than 8 (in powers of two), so O in TMEM is rescaled
-//    rarely; while one block's rows are in the softmax, the other's products
+//    rarely (P is kept 2^6 times as large as it is: below 2^14, and fp16 holds
+//    what is 2^-30 of the largest); while one block's rows are in the softmax, the other's products
 //    run.
 // Products are issued in the order P0 V(j), S0(j + 1), P1 V(j), S1(j + 1): a
 // commit after S t (j + 1) also says that O t holds all of tile j.
@@ -44,6 +48,7 @@ constexpr int kTile = 128;
 constexpr int kBlockRows = 256;
 constexpr uint32_t kAtom = 128 * 128; // 128 rows of 128 bytes
 constexpr int kErrPromptWait = 43;
+constexpr float kLift = 6.f; // log2 of the factor that P carries
 constexpr int kSplitCtas = 148;             // that share row blocks at most
 constexpr size_t kCounterBytes = (1 << 16) * 4; // as in the other kernel's workspace
 
@@ -187,8 +192,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kOffBars);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7;
   uint64_t *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 15, *drain = bars + 17; // p_full: block, half
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 18);
+  uint64_t *v_known = bars + 18, *e_full = bars + 19; // e_full by stage
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 21);
   volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  int *v_most = reinterpret_cast<int *>(tmem_slot + 2);          // by tile parity
+  volatile int *v_exp = reinterpret_cast<volatile int *>(v_most + 2); // by stage
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -204,6 +212,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
       mbar_init(o_full + i, 1);
     }
     mbar_init(drain, 1);
+    mbar_init(v_known, kRestoreWarps);
+    mbar_init(e_full, 1);
+    mbar_init(e_full + 1, 1);
+    v_most[0] = v_most[1] = -100;
     *abort = 0;
     fence_barrier_init();
   }
@@ -298,6 +310,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t t_s = tmem + lanes + block * 128, t_o = tmem + lanes + 256 + block * 128;
       float m = -INFINITY, l = 0.f;
+      int exponent = -100; // of O, for a bf16 cache
       for (int j = 0; j < tiles; ++j) {
         ok = mbar_wait(s_full + block, j & 1, abort);
         ok = __all_sync(~0u, ok);
@@ -343,10 +356,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]);
           }
         const float up = fmaxf(m, top * g.scale_log2);
-        if (__any_sync(~0u, up > m + 8.f)) {
-          const float f = up > m ? ex2_ftz(m - up) : 1.f;
+        int raise = 0; // of the values' power of two
+        if constexpr (BF16) {
+          ok = mbar_wait(e_full + (j & 1), (j / 2) & 1, abort);
+          ok = __all_sync(~0u, ok);
+          if (!ok)
+            break;
+          raise = v_exp[j & 1] - exponent;
+          exponent += raise;
+        }
+        if (raise || __any_sync(~0u, up > m + 8.f)) {
+          float f = up > m ? ex2_ftz(m - up) : 1.f;
           m = up;
           l *= f;
+          if (BF16)
+            f *= raise > 126 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - raise) << 23);
           if (j > 0) {
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
@@ -360,7 +384,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             }
           }
         }
-        const float minus = m == -INFINITY ? 0.f : -m;
+        const float minus = m == -INFINITY ? 0.f : kLift - m;
         float2 sum = make_float2(0.f, 0.f), sum2 = sum;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -388,7 +412,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
               if (i >= 2 * kApart) {
                 const int k = i - 2 * kApart;
                 fadd2(k & 1 ? sum2 : sum, x[k]);
-                p[k] = kv4_pack<BF16>(x[k].x, x[k].y);
+                p[k] = kv4_pack<false>(x[k].x, x[k].y);
               }
             }
           }
@@ -408,6 +432,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
       bool last = ok; // this warp writes its rows
       if (ok)
         tc_fence_after();
+      // Outputs are divided by their sum (nothing seen: 0; NaN stays NaN), and
+      // a bf16 cache's values get their power of two back.
+      const float own = (l > 0.f ? __fdividef(1.f, l) : l) *
+                        (BF16 ? __uint_as_float(static_cast<uint32_t>(127 + exponent) << 23) : 1.f);
       // Parts of this warp's 32 rows: [D] outputs, m and l, each [32].
       constexpr int kPart = (D + 2) * 32;
       float *const warp_parts = g.parts + static_cast<long long>(place) * g.splits * 8 * kPart + warp * kPart + lane;
@@ -421,7 +449,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            mine[(16 * c + e) * 32] = __uint_as_float(o[e]);
+            mine[(16 * c + e) * 32] = __uint_as_float(o[e]) * own;
         }
         mine[D * 32] = m;
         mine[(D + 1) * 32] = l;
@@ -448,7 +476,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         }
       }
       if (last) {
-        const float f = l > 0.f ? __fdividef(1.f, l) : l; // nothing seen: 0; NaN stays NaN
+        const float f = parts == 1 ? own : 1.f;
+        const float inverse = l > 0.f ? __fdividef(1.f, l) : l;
         // Through the rows' place of the queries, which all products have
         // read by now.
         auto stage = [&](int chunk, const uint32_t *o) {
@@ -477,18 +506,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
               v[e] = 0.f;
 #pragma unroll 1
             for (int i = 0; i < parts; i += 4) {
-              float x[4], y[4][16]; // four parts' loads at once
+              float x[4], z[4], y[4][16]; // four parts' loads at once
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const float *p = warp_parts + min(i + k, parts - 1) * next_part;
                 x[k] = __ldcg(p + D * 32);
+                z[k] = __ldcg(p + (D + 1) * 32);
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                   y[k][e] = __ldcg(p + (16 * c + e) * 32);
               }
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const float r = x[k] == -INFINITY || i + k >= parts ? 0.f : ex2_ftz(x[k] - m);
+                const float r = x[k] == -INFINITY || i + k >= parts ? 0.f : z[k] * ex2_ftz(x[k] - m) * inverse;
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                   v[e] = fmaf(y[k][e], r, v[e]);
@@ -532,6 +562,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
       uint32_t params[2][kMine];
       int ids[2][kMine]; // page of the piece's tokens in the tile to fetch next
       bool bad = false;
+      int exponent = -100; // a bf16 cache's values are divided by 2^exponent
       // Warps that take one more piece of the keys take one less of the values.
       auto piece_of = [&](int values, int i) { return (values ? kRestoreWarps - 1 - w : w) + i * kRestoreWarps; };
       auto token_of = [&](int values, int i) { return piece_of(values, i) * kTokens + tok0; };
@@ -560,7 +591,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         const uint4 code = codes[values][i];
         // Past the length: zeros.
         const uint32_t group = key_of_tile(j) + tok < seq.len ? params[values][i] : 0u;
-        const uint32_t scale = __byte_perm(group, 0, 0x1010), low = __byte_perm(group, 0, 0x3232);
+        uint32_t scale, low;
+        if (BF16 && values) {
+          const float down = __uint_as_float(static_cast<uint32_t>(127 - exponent) << 23);
+          scale = kv4_pack<false>(kv4_lo<true>(group) * down, kv4_lo<true>(group) * down);
+          low = kv4_pack<false>(kv4_hi<true>(group) * down, kv4_hi<true>(group) * down);
+        } else {
+          scale = __byte_perm(group, 0, 0x1010);
+          low = __byte_perm(group, 0, 0x3232);
+        }
         // Lanes of the upper two groups write their chunks in another order,
         // so that the eight lanes of a phase meet eight bank columns.
         const bool turn = c >= 2;
@@ -570,7 +609,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int chunk = (c & 1) * 4 + (turn ? e ^ 2 : e);
-          sts_v4(row + ((chunk ^ (tok & 7)) << 4), restore_row<BF16>(in[e], scale, low));
+          sts_v4(row + ((chunk ^ (tok & 7)) << 4),
+                 values ? restore_row<false>(in[e], scale, low) : restore_row<BF16>(in[e], scale, low));
         }
       };
 #pragma unroll
@@ -587,6 +627,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         const int st = j & 1;
 #pragma unroll
         for (int values = 0; values < 2; ++values) {
+          if (BF16 && values) {
+            // The largest exponent of the tile's value parameters (16 scale and
+            // minimum: a value is below four times that), for all warps.
+            int most = exponent;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i)
+              if (piece_of(1, i) < kPieces && key_of_tile(j) + token_of(1, i) < seq.len) {
+                const uint32_t g1 = params[1][i] & 0x7FFF7FFFu;
+                most = max(most, max(static_cast<int>(g1 >> 7 & 0xFFu) + 4, static_cast<int>(g1 >> 23)) - 127);
+              }
+            most = __reduce_max_sync(~0u, most);
+            if (lane == 0) {
+              atomicMax(v_most + st, most);
+              mbar_arrive(v_known);
+            }
+            ok = mbar_wait(v_known, j & 1, abort);
+            ok = __all_sync(~0u, ok);
+            if (!ok)
+              break;
+            // The other tile's slot is in use only once every warp is past
+            // this one. Small changes are left to fp16's own range.
+            most = min(*reinterpret_cast<volatile int *>(v_most + st), 120);
+            exponent = most > exponent + 12 ? most : exponent;
+          }
           if (j >= 2) {
             ok = mbar_wait((values ? v_empty : k_empty) + st, (j / 2 - 1) & 1, abort);
             ok = __all_sync(~0u, ok);
@@ -594,6 +658,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
               break;
           }
           const uint32_t operand = sbase + (values ? L::kOffV : L::kOffK) + st * L::kOperand;
+          if (BF16 && values && w == 0 && lane == 0) {
+            v_exp[st] = exponent;
+            mbar_arrive(e_full + st);
+          }
 #pragma unroll
           for (int i = 0; i < kMine; ++i)
             if (piece_of(values, i) < kPieces)
@@ -615,7 +683,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
       // ------------------------------------------------------------- issuing
       constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
       constexpr uint32_t idesc_s = idesc_f16_f32(128, 128) | kType;
-      constexpr uint32_t idesc_o = idesc_f16_f32(128, D) | kType | (1u << 16); // B is MN-major
+      constexpr uint32_t idesc_o = idesc_f16_f32(128, D) | (1u << 16); // fp16, B is MN-major
       auto scores = [&](int block, int st) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {

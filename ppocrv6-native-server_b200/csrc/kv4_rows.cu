@@ -23,13 +23,18 @@
 //    rows are scaled by a power of two to just below 2^14 first (exact, and
 //    bf16 queries fit fp16 this way). A group's dot product becomes
 //    scale * (q . c) + minimum * sum(q) in fp32.
-//  * P^T in 16 bits (p is at most 2^8, see below; rounding it costs 2^-12 or
-//    2^-9 relative per term, the precision of the output's own type);
+//  * P^T in fp16 (p is at most 2^14, see below; rounding it costs 2^-12
+//    relative per term, the precision of an fp16 output);
 //    movmatrix turns it into the second product's operand.
-//  * O^T = V^T P^T with the values restored to 16 bits: minimum + scale * c
-//    rounded once, again the precision of the cache's type.
+//  * O^T = V^T P^T with the values restored to fp16: minimum + scale * c
+//    rounded once, again 2^-12 relative. A bf16 cache's values are restored
+//    divided by a power of two that follows the largest parameters met, so
+//    that they fit fp16 (what is lost lies 2^-25 below the largest) and keep
+//    three bits more than bf16 would.
 // The running maximum is only raised when a score passes it by more than 8
-// (in powers of two): until then p stays below 2^8 and nothing is rescaled.
+// (in powers of two): until then nothing is rescaled. p is kept 2^6 times as
+// large as it is, so that it stays below 2^14 and fp16 holds what is 2^-30 of
+// the largest.
 //
 // Keys past a sequence's length are never used: their scores are replaced
 // (not multiplied) and their values' parameters zeroed, so a page may hold
@@ -51,6 +56,7 @@ constexpr int kMaxUnits = 1 << 16; // counters in the workspace
 constexpr int kMaxCtas = 148 * 3;
 constexpr int kPartFloats = 16 * (128 + 2);
 constexpr int kErrRowsWait = 42;
+constexpr float kLift = 6.f; // log2 of the factor that p carries
 
 struct RowsArgs {
   Kv4Tokens t;
@@ -79,12 +85,6 @@ __device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)
                "{%10,%10,%10,%10};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -216,36 +216,24 @@ template <int D> __device__ __forceinline__ int order(int k) {
   return D == 128 ? ((k >> 1) & 1) + (k >> 2) * 4 + (k & 1) * 2 : (k >> 1) + (k & 1) * 4;
 }
 
-// Four channels of two keys (16-bit lanes a, b of x): values rounded to the
-// cache's type.
-template <bool BF16>
+// Four channels of two keys (16-bit lanes a, b of x): fp16 values.
 __device__ __forceinline__ void restore4(uint32_t x, uint32_t scale, uint32_t low, uint32_t (&v)[4]) {
-  if constexpr (BF16) {
-    const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162 *>(&scale);
-    const __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162 *>(&low);
-    const uint32_t off = 0x43004300u; // 128 + c
-    const __nv_bfloat162 o = *reinterpret_cast<const __nv_bfloat162 *>(&off);
+  const __half2 s = *reinterpret_cast<const __half2 *>(&scale);
+  const __half2 m = *reinterpret_cast<const __half2 *>(&low);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t c = ((x >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-      const __nv_bfloat162 r = __hfma2(__hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&c), o), s, m);
-      v[i] = *reinterpret_cast<const uint32_t *>(&r);
-    }
-  } else {
-    const __half2 s = *reinterpret_cast<const __half2 *>(&scale);
-    const __half2 m = *reinterpret_cast<const __half2 *>(&low);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t y = i < 2 ? x : x >> 8;
-      const uint32_t c = (y & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u; // 1024 + c or 1024 + 16 c
-      const __half2 w = *reinterpret_cast<const __half2 *>(&c);
-      const __half2 n = i & 1 ? __hfma2(w, __float2half2_rn(0.0625f), __float2half2_rn(-64.f))
-                              : __hsub2(w, __float2half2_rn(1024.f));
-      const __half2 r = __hfma2(n, s, m);
-      v[i] = *reinterpret_cast<const uint32_t *>(&r);
-    }
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t y = i < 2 ? x : x >> 8;
+    const uint32_t c = (y & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u; // 1024 + c or 1024 + 16 c
+    const __half2 w = *reinterpret_cast<const __half2 *>(&c);
+    const __half2 n = i & 1 ? __hfma2(w, __float2half2_rn(0.0625f), __float2half2_rn(-64.f))
+                            : __hsub2(w, __float2half2_rn(1024.f));
+    const __half2 r = __hfma2(n, s, m);
+    v[i] = *reinterpret_cast<const uint32_t *>(&r);
   }
 }
+
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float power2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
 template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
@@ -494,6 +482,7 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
 
     float o[kTiles][NT][4];
     float m[NT][2], l[NT][2];
+    int v_exp = -100; // a bf16 cache's values are divided by 2^v_exp
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -623,7 +612,8 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         // Nothing seen yet: every score is -inf, and so must its power be 0.
-        const float m0 = m[nt][0] == -INFINITY ? 0.f : -m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : -m[nt][1];
+        const float m0 = m[nt][0] == -INFINITY ? 0.f : kLift - m[nt][0];
+        const float m1 = m[nt][1] == -INFINITY ? 0.f : kLift - m[nt][1];
         const float f0 = factor[nt][0], f1 = factor[nt][1];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -631,9 +621,46 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
           const float p2 = ex2_ftz(fmaf(s[h][nt][2], f0, m0)), p3 = ex2_ftz(fmaf(s[h][nt][3], f1, m1));
           l[nt][0] += p0 + p2;
           l[nt][1] += p1 + p3;
-          pf[h][nt][0] = transpose8x8(kv4_pack<BF16>(p0, p1));
-          pf[h][nt][1] = transpose8x8(kv4_pack<BF16>(p2, p3));
+          pf[h][nt][0] = transpose8x8(kv4_pack<false>(p0, p1));
+          pf[h][nt][1] = transpose8x8(kv4_pack<false>(p2, p3));
         }
+      }
+      // The values' parameters of this lane's channels: slice, pair, key.
+      uint32_t vp[2][2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          vp[h][u][0] = lds_u32(st + v_groups_a[h] + 8 * u * (D / 8));
+          vp[h][u][1] = lds_u32(st + v_groups_b[h] + 8 * u * (D / 8));
+          if (!clear) {
+            const int key = key0 + h * 16 + 8 * u;
+            vp[h][u][0] = key + key_a < x.s.len ? vp[h][u][0] : 0u;
+            vp[h][u][1] = key + key_b < x.s.len ? vp[h][u][1] : 0u;
+          }
+        }
+      float v_scale = 1.f;
+      if constexpr (BF16) {
+        uint32_t most = 0; // largest magnitudes: scale | minimum
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          most = __vmaxu2(most, vp[i / 4][i / 2 % 2][i % 2] & 0x7FFF7FFFu);
+        // Exponent of 16 scale and of the minimum: a value is below four
+        // times the larger one.
+        const int ex = max(static_cast<int>(most >> 7 & 0xFFu) + 4, static_cast<int>(most >> 23)) - 127;
+        if (__any_sync(~0u, ex > v_exp + 12)) {
+          const int up = min(__reduce_max_sync(~0u, ex), 120);
+          const float r = v_exp - up < -126 ? 0.f : power2(min(v_exp - up, 0));
+#pragma unroll
+          for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                o[d][nt][i] *= r;
+          v_exp = max(v_exp, up);
+        }
+        v_scale = power2(-v_exp);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -641,15 +668,14 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
         uint32_t scale[2], low[2], w[2][2][D == 128 ? 2 : 1];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int ka = key_a + 8 * u, kb = key_b + 8 * u;
-          uint32_t pa = lds_u32(st + v_groups_a[h] + 8 * u * (D / 8)), pb = lds_u32(st + v_groups_b[h] + 8 * u * (D / 8));
-          if (!clear) {
-            const int key = key0 + h * 16;
-            pa = key + ka < x.s.len ? pa : 0u;
-            pb = key + kb < x.s.len ? pb : 0u;
+          const uint32_t pa = vp[h][u][0], pb = vp[h][u][1];
+          if constexpr (BF16) {
+            scale[u] = kv4_pack<false>(kv4_lo<true>(pa) * v_scale, kv4_lo<true>(pb) * v_scale);
+            low[u] = kv4_pack<false>(kv4_hi<true>(pa) * v_scale, kv4_hi<true>(pb) * v_scale);
+          } else {
+            scale[u] = __byte_perm(pa, pb, 0x5410);
+            low[u] = __byte_perm(pa, pb, 0x7632);
           }
-          scale[u] = __byte_perm(pa, pb, 0x5410);
-          low[u] = __byte_perm(pa, pb, 0x7632);
           const uint32_t ra = st + v_codes_a[h] + 8 * u * (D / 2), rb = st + v_codes_b[h] + 8 * u * (D / 2);
           if constexpr (D == 128) {
             const uint2 a = lds_v2(ra), c = lds_v2(rb);
@@ -666,17 +692,14 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
         if constexpr (D == 32) {
           // Channels 4 lr .. 4 lr + 3: tile t takes t and t + 2.
           uint32_t v0[4], v1[4];
-          restore4<BF16>(__byte_perm(w[0][0][0], w[0][1][0], 0x5410), scale[0], low[0], v0);
-          restore4<BF16>(__byte_perm(w[1][0][0], w[1][1][0], 0x5410), scale[1], low[1], v1);
+          restore4(__byte_perm(w[0][0][0], w[0][1][0], 0x5410), scale[0], low[0], v0);
+          restore4(__byte_perm(w[1][0][0], w[1][1][0], 0x5410), scale[1], low[1], v1);
 #pragma unroll
           for (int d = 0; d < 2; ++d) {
             const uint32_t a[4] = {v0[d], v0[d + 2], v1[d], v1[d + 2]};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              if constexpr (BF16)
-                mma_bf16(o[d][nt], a, pf[h][nt][0], pf[h][nt][1]);
-              else
-                mma_f16(o[d][nt], a, pf[h][nt][0], pf[h][nt][1]);
+              mma_f16(o[d][nt], a, pf[h][nt][0], pf[h][nt][1]);
             }
           }
         } else {
@@ -685,19 +708,16 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
 #pragma unroll
           for (int i = 0; i < D / 64; ++i) {
             uint32_t v0[4], v1[4], v2[4], v3[4];
-            restore4<BF16>(__byte_perm(w[0][0][i], w[0][1][i], 0x5410), scale[0], low[0], v0);
-            restore4<BF16>(__byte_perm(w[0][0][i], w[0][1][i], 0x7632), scale[0], low[0], v1);
-            restore4<BF16>(__byte_perm(w[1][0][i], w[1][1][i], 0x5410), scale[1], low[1], v2);
-            restore4<BF16>(__byte_perm(w[1][0][i], w[1][1][i], 0x7632), scale[1], low[1], v3);
+            restore4(__byte_perm(w[0][0][i], w[0][1][i], 0x5410), scale[0], low[0], v0);
+            restore4(__byte_perm(w[0][0][i], w[0][1][i], 0x7632), scale[0], low[0], v1);
+            restore4(__byte_perm(w[1][0][i], w[1][1][i], 0x5410), scale[1], low[1], v2);
+            restore4(__byte_perm(w[1][0][i], w[1][1][i], 0x7632), scale[1], low[1], v3);
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
               const uint32_t a[4] = {v0[d], v1[d], v2[d], v3[d]};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                if constexpr (BF16)
-                  mma_bf16(o[4 * i + d][nt], a, pf[h][nt][0], pf[h][nt][1]);
-                else
-                  mma_f16(o[4 * i + d][nt], a, pf[h][nt][0], pf[h][nt][1]);
+                mma_f16(o[4 * i + d][nt], a, pf[h][nt][0], pf[h][nt][1]);
               }
             }
           }
@@ -722,6 +742,17 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
         }
       }
     consumer_barrier();
+    auto row_stats = [&](int row, float &top, float &sum) {
+      top = stat_m[row];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w)
+        top = fmaxf(top, stat_m[w * kRows + row]);
+      sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        sum += top == -INFINITY ? 0.f : stat_l[w * kRows + row] * ex2_ftz(stat_m[w * kRows + row] - top);
+    };
+    auto inverse_of = [](float sum) { return sum > 0.f ? __fdividef(1.f, sum) : sum; }; // NaN stays NaN
     // Warps 2 and 3 leave theirs, warps 0 and 1 add their own to it.
 #pragma unroll
     for (int half = 1; half >= 0; --half) {
@@ -731,11 +762,11 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int row = nt * 8 + 2 * lc + i;
-            float top = stat_m[row];
-#pragma unroll
-            for (int w = 1; w < kWarps; ++w)
-              top = fmaxf(top, stat_m[w * kRows + row]);
-            const float r = m[nt][i] == -INFINITY ? 0.f : ex2_ftz(m[nt][i] - top);
+            float top, sum;
+            row_stats(row, top, sum);
+            // Outputs are divided by their sum here, and a bf16 cache's
+            // values get their power of two back.
+            const float r = m[nt][i] == -INFINITY ? 0.f : ex2_ftz(m[nt][i] - top) * inverse_of(sum) * (BF16 ? power2(v_exp) : 1.f);
             // This thread's channels of the row are D / 8 neighbours.
             float4 *dst = reinterpret_cast<float4 *>(merge + ((warp & 1) * kRows + row) * D + lr * (D / 8));
             float v[D / 8];
@@ -773,20 +804,13 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
       float4 v = *reinterpret_cast<const float4 *>(merge + row * D + d);
       const float4 y = *reinterpret_cast<const float4 *>(merge + (kRows + row) * D + d);
       v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
-      float top = stat_m[row];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w)
-        top = fmaxf(top, stat_m[w * kRows + row]);
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-        sum += top == -INFINITY ? 0.f : stat_l[w * kRows + row] * ex2_ftz(stat_m[w * kRows + row] - top);
       if (whole) {
-        const float r = sum > 0.f ? __fdividef(1.f, sum) : sum; // NaN stays NaN
-        store(row, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
+        store(row, d, v);
       } else {
         *reinterpret_cast<float4 *>(part + row * D + d) = v;
         if (d == 0) {
+          float top, sum;
+          row_stats(row, top, sum);
           part[kRows * D + row] = top;
           part[kRows * D + kRows + row] = sum;
         }
@@ -812,32 +836,58 @@ __global__ void __launch_bounds__(kRowsThreads, (RowsLayout<D, NT>::kCtasPerSm))
           // The unit's first CTA went out on it, the others came in.
           return g.parts + static_cast<long long>((first + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats;
         };
-        // Largest maximum of each row, by 32 kWarps / kRows threads each.
+        // Largest maximum and total of each row, by kBy threads each; the
+        // parts' shares stay in shared memory where they fit.
+        constexpr int kBy = 32 * kWarps / kRows, kStaged = (L::kMergeFloats - 64 * kWarps) / kRows;
+        float *totals = merge + 32 * kWarps, *shares = merge + 64 * kWarps;
+        const int own = tid % kRows;
+        auto stat_of = [&](int i, int row, int which) { return __ldcg(part_of(i) + kRows * D + which * kRows + row); };
         float best = -INFINITY;
 #pragma unroll 4
-        for (int i = tid / kRows; i < parts; i += 32 * kWarps / kRows)
-          best = fmaxf(best, __ldcg(part_of(i) + kRows * D + tid % kRows));
+        for (int i = tid / kRows; i < parts; i += kBy)
+          best = fmaxf(best, stat_of(i, own, 0));
         merge[tid] = best;
+        consumer_barrier();
+        auto top_of = [&](int row) {
+          float top = merge[row];
+#pragma unroll
+          for (int i = 1; i < kBy; ++i)
+            top = fmaxf(top, merge[i * kRows + row]);
+          return top;
+        };
+        auto share_of = [&](int i, int row, float top) {
+          const float x = stat_of(i, row, 0);
+          return x == -INFINITY ? 0.f : stat_of(i, row, 1) * ex2_ftz(x - top);
+        };
+        {
+          const float top = top_of(own);
+          float total = 0.f;
+#pragma unroll 4
+          for (int i = tid / kRows; i < parts; i += kBy) {
+            const float x = share_of(i, own, top);
+            total += x;
+            if (i < kStaged)
+              shares[i * kRows + own] = x;
+          }
+          totals[tid] = total;
+        }
         consumer_barrier();
         for (int it = tid; it < kRows * D / 4; it += 32 * kWarps) {
           const int row = it / (D / 4), d = it % (D / 4) * 4;
-          float top = merge[row];
+          const float top = top_of(row);
+          float total = 0.f;
 #pragma unroll
-          for (int i = 1; i < 32 * kWarps / kRows; ++i)
-            top = fmaxf(top, merge[i * kRows + row]);
-          float sum = 0.f;
+          for (int i = 0; i < kBy; ++i)
+            total += totals[i * kRows + row];
+          total = inverse_of(total);
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
           for (int i = 0; i < parts; ++i) {
-            const float *p = part_of(i);
-            const float4 y = __ldcg(reinterpret_cast<const float4 *>(p + row * D + d));
-            const float my = __ldcg(p + kRows * D + row), ly = __ldcg(p + kRows * D + kRows + row);
-            const float r = my == -INFINITY ? 0.f : ex2_ftz(my - top);
-            sum += ly * r;
+            const float4 y = __ldcg(reinterpret_cast<const float4 *>(part_of(i) + row * D + d));
+            const float r = (i < kStaged ? shares[i * kRows + row] : share_of(i, row, top)) * total;
             v.x += y.x * r, v.y += y.y * r, v.z += y.z * r, v.w += y.w * r;
           }
-          const float r = sum > 0.f ? __fdividef(1.f, sum) : sum;
-          store(row, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
+          store(row, d, v);
         }
       }
     }

@@ -376,6 +376,34 @@ def test_attention_small_and_large_queries(native, cuda, dtype):
     assert ((o - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("new", [1, 80])
+@pytest.mark.parametrize("sizes", [[1e-30, 1e-3, 1.0, 1e15, 1e30], [1e30, 1.0, 1e-30], [0.0, 0.0, 1e-35], [3e37, 3e37]])
+def test_attention_bf16_values_of_any_size(native, cuda, new, sizes):
+    """bf16 values far beyond fp16's range, growing and shrinking along the cache."""
+    s = Scene([900], [new], 2, 64, 64, BF16, seed=13)
+    each = -(-900 // len(sizes))
+    s.v[0] = (s.v[0].float().clamp(-2, 2) * torch.tensor(sizes).repeat_interleave(each)[:900, None, None]).to(BF16)
+    check_attention(native, s, 4, keys_rounded=new > 1, rows={0, 40})
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_many_light_keys(native, cuda, dtype):
+    """One key far above thousands of light ones, whose shares together count."""
+    n = 6000
+    s = Scene([n], [1], 1, 32, 128, dtype, seed=14)
+    s.k[0] = torch.zeros(n, 1, 32).to(dtype)
+    s.k[0][7] = 1.0
+    s.v[0] = (torch.ones(n, 1, 32) + 0.25 * torch.randn(n, 1, 32, generator=gen(15))).to(dtype)
+    s.fill([n])
+    cache = s.cache()
+    q = torch.full((1, 1, 32), 14 / 32, dtype=dtype)
+    got = cache.attention(q.cuda(), *s.places(), scale=1.0).cpu().double()
+    assert fault(native) == 0
+    k, v = (O.held(s.pool, 128, 32, dtype, s.table[0], n, w) for w in (0, 1))
+    want, mag, most = O.attention(q, k, v, n - 1, 1.0)
+    assert ((got - want).abs() <= mag * (3.2 * U[dtype] + math.expm1(2.2 * 2.0 ** -20 * float(most.max())))).all()
+
+
 def test_attention_nan_query_stays_in_its_row(native, cuda):
     s = Scene([100, 50], [1, 1], 2, 64, 16, F16, seed=6)
     s.fill([100, 50])
