@@ -22,7 +22,7 @@ extern "C" {
 enum { PPOCR_B200_F16 = 0, PPOCR_B200_BF16 = 1, PPOCR_B200_F32 = 2 };
 
 // A cache of `pages` pages of page_size tokens (16, 32, 64 or 128) for
-// kv_heads heads of head_dim channels (32, 64 or 128), in a pool of
+// kv_heads (at most 4096) heads of head_dim channels (32, 64 or 128), in a pool of
 // pages * kv_heads * ppocr_b200_kv4_block_bytes() bytes, 16-byte aligned.
 // One (page, head) block holds, with G = head_dim / 32 groups per token:
 //   key codes    [page_size][head_dim / 2]  two channels a byte, the even one
@@ -49,6 +49,7 @@ size_t ppocr_b200_kv4_block_bytes(int page_size, int head_dim);
 //                                 starts[b + 1] - 1 of the packed arrays; null:
 //                                 max_new each (tokens = batch * max_new)
 //   tokens  rows of the packed arrays; max_new: no sequence has more new ones
+//           (rows that belong to no sequence are left as they are)
 // A new token whose position would be negative (more new tokens than the
 // length) is not written, reads back as zero and sees no key.
 

@@ -8,6 +8,7 @@
 #include "../../include/ppocr_b200_preprocess.h"
 #include "kernels.h"
 #include <algorithm>
+#include <exception>
 #include <map>
 #include <mutex>
 #include <string>
@@ -66,6 +67,21 @@ void *stream_workspace(size_t bytes, cudaStream_t stream) {
 
 size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
+// Runs an entry point's body; nothing is thrown past the C boundary.
+template <typename Body> int guarded(Body body) {
+  try {
+    g_error.clear();
+    return body();
+  } catch (const std::exception &e) {
+    try {
+      return fail(e.what());
+    } catch (...) {
+    }
+  } catch (...) {
+  }
+  return -1;
+}
+
 bool aligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 // Checks what the three cache calls share. Returns null, or what is wrong.
@@ -77,8 +93,9 @@ const char *kv4_arguments(const PpocrKv4Cache *cache, const int *table, int widt
     return "cache type must be f16 or bf16";
   if (!ppocr_b200_kv4_block_bytes(cache->page_size, cache->head_dim))
     return "page size must be 16, 32, 64 or 128 and head_dim 32, 64 or 128";
-  if (cache->kv_heads <= 0 || cache->pages <= 0 || cache->pages > ((1ll << 31) - 1) / cache->kv_heads)
-    return "pages and kv_heads must be positive, pages * kv_heads below 2^31";
+  if (cache->kv_heads <= 0 || cache->kv_heads > 4096 || cache->pages <= 0 ||
+      cache->pages > ((1ll << 31) - 1) / cache->kv_heads)
+    return "kv_heads must be 1 to 4096, pages positive, pages * kv_heads below 2^31";
   if (batch < 0 || batch > 65535 || tokens < 0 || max_new < 0)
     return "batch (at most 65535), tokens and max_new must not be negative";
   if (!table || !lengths || width <= 0 || width >= (1 << 30) / cache->page_size)
@@ -749,39 +766,41 @@ size_t ppocr_b200_kv4_block_bytes(int page_size, int head_dim) {
 int ppocr_b200_kv4_append(const PpocrKv4Cache *cache, const void *k, long long k_stride, const void *v,
                           long long v_stride, const int *table, int width, const int *lengths, const int *starts,
                           int batch, int tokens, int max_new, cudaStream_t stream) {
-  g_error.clear();
-  Kv4Cache c;
-  Kv4Tokens t;
-  const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
-  if (!bad)
-    bad = kv4_row_arguments(cache, max_new);
-  if (bad)
-    return fail(std::string("kv4 append: ") + bad);
-  if (batch == 0 || tokens == 0 || max_new == 0)
-    return 0;
-  const long long row = static_cast<long long>(c.kv_heads) * c.head_dim;
-  if (!k || !v || !aligned(k, 16) || !aligned(v, 16) || k_stride < row || v_stride < row || k_stride % 8 ||
-      v_stride % 8)
-    return fail("kv4 append: k and v must be 16-byte aligned, with row strides of at least a row and a multiple of 8");
-  return status(kv4_append(c, t, k, k_stride, v, v_stride, stream), "kv4 append");
+  return guarded([&]() -> int {
+    Kv4Cache c;
+    Kv4Tokens t;
+    const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
+    if (!bad)
+      bad = kv4_row_arguments(cache, max_new);
+    if (bad)
+      return fail(std::string("kv4 append: ") + bad);
+    if (batch == 0 || tokens == 0 || max_new == 0)
+      return 0;
+    const long long row = static_cast<long long>(c.kv_heads) * c.head_dim;
+    if (!k || !v || !aligned(k, 16) || !aligned(v, 16) || k_stride < row || v_stride < row || k_stride % 8 ||
+        v_stride % 8)
+      return fail("kv4 append: k and v must be 16-byte aligned, with row strides of at least a row and a multiple of 8");
+    return status(kv4_append(c, t, k, k_stride, v, v_stride, stream), "kv4 append");
+  });
 }
 
 int ppocr_b200_kv4_read(const PpocrKv4Cache *cache, void *k, void *v, const int *table, int width,
                         const int *lengths, const int *starts, int batch, int tokens, int max_new,
                         cudaStream_t stream) {
-  g_error.clear();
-  Kv4Cache c;
-  Kv4Tokens t;
-  const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
-  if (!bad)
-    bad = kv4_row_arguments(cache, max_new);
-  if (bad)
-    return fail(std::string("kv4 read: ") + bad);
-  if (batch == 0 || tokens == 0 || max_new == 0)
-    return 0;
-  if (!k || !v || !aligned(k, 16) || !aligned(v, 16))
-    return fail("kv4 read: k and v must be 16-byte aligned");
-  return status(kv4_read(c, t, k, v, stream), "kv4 read");
+  return guarded([&]() -> int {
+    Kv4Cache c;
+    Kv4Tokens t;
+    const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
+    if (!bad)
+      bad = kv4_row_arguments(cache, max_new);
+    if (bad)
+      return fail(std::string("kv4 read: ") + bad);
+    if (batch == 0 || tokens == 0 || max_new == 0)
+      return 0;
+    if (!k || !v || !aligned(k, 16) || !aligned(v, 16))
+      return fail("kv4 read: k and v must be 16-byte aligned");
+    return status(kv4_read(c, t, k, v, stream), "kv4 read");
+  });
 }
 
 size_t ppocr_b200_kv4_workspace_bytes(void) {
@@ -792,71 +811,73 @@ int ppocr_b200_kv4_attention(const PpocrKv4Cache *cache, const void *q, long lon
                              float scale, int window, int sinks, const int *table, int width, const int *lengths,
                              const int *starts, int batch, int tokens, int max_new, void *workspace,
                              cudaStream_t stream) {
-  g_error.clear();
-  Kv4Cache c;
-  Kv4Tokens t;
-  const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
-  if (bad)
-    return fail(std::string("kv4 attention: ") + bad);
-  if (heads <= 0 || heads % c.kv_heads)
-    return fail("kv4 attention: heads must be a multiple of kv_heads");
-  if (static_cast<long long>(max_new) * (heads / c.kv_heads) >= (1ll << 30) ||
-      static_cast<long long>(max_new) * heads / 256 * batch >= (1ll << 30))
-    return fail("kv4 attention: batch * max_new * heads is too large");
-  if (window < 0 || sinks < 0 || !(scale - scale == 0.f))
-    return fail("kv4 attention: window and sinks must not be negative, scale must be finite");
-  if (batch == 0 || tokens == 0 || max_new == 0)
-    return 0;
-  if (!q || !out || !aligned(q, 16) || !aligned(out, 16) || q_stride % 8 ||
-      q_stride < static_cast<long long>(heads) * c.head_dim)
-    return fail("kv4 attention: q and out must be 16-byte aligned, q's row stride at least a row and a multiple of 8");
-  if (!workspace || !aligned(workspace, 256))
-    return fail("kv4 attention: workspace missing or not 256-byte aligned");
-  Kv4Attention a;
-  a.q = q;
-  a.out = out;
-  a.q_stride = q_stride;
-  a.heads = heads;
-  a.window = window;
-  a.sinks = sinks;
-  a.scale = scale;
-  a.workspace = workspace;
-  // Up to 32 query rows per (sequence, key head) read the cache with as many
-  // CTAs as there are tiles for; more share restored tiles on tcgen05.
-  // Measured, heads of 128: 16 sequences of 8000 keys at 32 rows 75 against
-  // 119 us, of 2000 keys at 64 rows 47 against 33 us.
-  const long long rows = static_cast<long long>(max_new) * (heads / c.kv_heads);
-  return status(rows <= 32 ? kv4_attend_rows(c, t, a, stream) : kv4_attend_prompt(c, t, a, stream), "kv4 attention");
+  return guarded([&]() -> int {
+    Kv4Cache c;
+    Kv4Tokens t;
+    const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
+    if (bad)
+      return fail(std::string("kv4 attention: ") + bad);
+    if (heads <= 0 || heads > 65536 || heads % c.kv_heads)
+      return fail("kv4 attention: heads must be a multiple of kv_heads (at most 65536)");
+    if (static_cast<long long>(max_new) * (heads / c.kv_heads) >= (1ll << 30) ||
+        static_cast<long long>(max_new) * heads / 256 * batch >= (1ll << 30))
+      return fail("kv4 attention: batch * max_new * heads is too large");
+    if (window < 0 || sinks < 0 || !(scale - scale == 0.f))
+      return fail("kv4 attention: window and sinks must not be negative, scale must be finite");
+    if (batch == 0 || tokens == 0 || max_new == 0)
+      return 0;
+    if (!q || !out || !aligned(q, 16) || !aligned(out, 16) || q_stride % 8 ||
+        q_stride < static_cast<long long>(heads) * c.head_dim)
+      return fail("kv4 attention: q and out must be 16-byte aligned, q's row stride at least a row and a multiple of 8");
+    if (!workspace || !aligned(workspace, 256))
+      return fail("kv4 attention: workspace missing or not 256-byte aligned");
+    Kv4Attention a;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.heads = heads;
+    a.window = window;
+    a.sinks = sinks;
+    a.scale = scale;
+    a.workspace = workspace;
+    // Up to 32 query rows per (sequence, key head) read the cache with as many
+    // CTAs as there are tiles for; more share restored tiles on tcgen05.
+    // Measured, heads of 128: 16 sequences of 8000 keys at 32 rows 75 against
+    // 119 us, of 2000 keys at 64 rows 47 against 33 us.
+    const long long rows = static_cast<long long>(max_new) * (heads / c.kv_heads);
+    return status(rows <= 32 ? kv4_attend_rows(c, t, a, stream) : kv4_attend_prompt(c, t, a, stream), "kv4 attention");
+  });
 }
 
 int ppocr_b200_sample(const void *logits, int type, long long stride, int rows, int vocab, const float *temperature,
                       const int *top_k, const float *top_p, const float *min_p, const float *uniform, int *ids,
                       float *prob, int *kept, cudaStream_t stream) {
-  g_error.clear();
-  if (type != PPOCR_B200_F16 && type != PPOCR_B200_BF16 && type != PPOCR_B200_F32)
-    return fail("sample: type must be f16, bf16 or f32");
-  // A row's mass is at most vocab * 2^32 and has to fit 63 bits with room.
-  if (rows < 0 || vocab <= 0 || vocab > (1 << 24) || stride < vocab)
-    return fail("sample: rows, vocab (at most 2^24) or stride out of range");
-  if (rows == 0)
-    return 0;
-  const size_t size = type == PPOCR_B200_F32 ? 4 : 2;
-  if (!logits || !aligned(logits, size) || !uniform || !ids || !prob || !kept)
-    return fail("sample: logits, uniform, ids, prob or kept missing or misaligned");
-  SampleArgs a;
-  a.logits = logits;
-  a.stride = stride;
-  a.rows = rows;
-  a.vocab = vocab;
-  a.temperature = temperature;
-  a.top_k = top_k;
-  a.top_p = top_p;
-  a.min_p = min_p;
-  a.uniform = uniform;
-  a.ids = ids;
-  a.prob = prob;
-  a.kept = kept;
-  return status(sample_tokens(a, type, stream), "sample");
+  return guarded([&]() -> int {
+    if (type != PPOCR_B200_F16 && type != PPOCR_B200_BF16 && type != PPOCR_B200_F32)
+      return fail("sample: type must be f16, bf16 or f32");
+    // A row's mass is at most vocab * 2^32 and has to fit 63 bits with room.
+    if (rows < 0 || vocab <= 0 || vocab > (1 << 24) || stride < vocab)
+      return fail("sample: rows, vocab (at most 2^24) or stride out of range");
+    if (rows == 0)
+      return 0;
+    const size_t size = type == PPOCR_B200_F32 ? 4 : 2;
+    if (!logits || !aligned(logits, size) || !uniform || !ids || !prob || !kept)
+      return fail("sample: logits, uniform, ids, prob or kept missing or misaligned");
+    SampleArgs a;
+    a.logits = logits;
+    a.stride = stride;
+    a.rows = rows;
+    a.vocab = vocab;
+    a.temperature = temperature;
+    a.top_k = top_k;
+    a.top_p = top_p;
+    a.min_p = min_p;
+    a.uniform = uniform;
+    a.ids = ids;
+    a.prob = prob;
+    a.kept = kept;
+    return status(sample_tokens(a, type, stream), "sample");
+  });
 }
 
 } // extern "C"

@@ -41,8 +41,8 @@ namespace {
 constexpr int kPromptThreads = 16 * 32; // 2 x 4 softmax warps, 7 restoring, 1 issuing
 constexpr int kRestoreWarps = 7;
 // Registers a thread: launched with 128, of which the two warpgroups of
-// restoring and issuing warps keep 80 and the two of softmax warps get 176.
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kOtherRegs = 80;
+// restoring and issuing warps keep 88 and the two of softmax warps get 168.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kOtherRegs = 88;
 static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "taken from the launch's own registers");
 constexpr int kTile = 128;
 constexpr int kBlockRows = 256;

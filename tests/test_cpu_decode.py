@@ -44,6 +44,7 @@ PLACES = dict(table=0x2000, width=4, lengths=0x3000, starts=0x4000, batch=2, tok
     (dict(page_size=48), {}, "page size"),
     (dict(head_dim=96), {}, "head_dim"),
     (dict(kv_heads=0), {}, "kv_heads"),
+    (dict(kv_heads=4097), {}, "kv_heads"),
     (dict(pages=1 << 31), {}, "2^31"),
     ({}, dict(table=None), "table"),
     ({}, dict(lengths=None), "lengths"),
@@ -87,7 +88,7 @@ def test_row_arguments():
     assert lib.ppocr_b200_kv4_read(c, None, 0x6000, *p, None) == -1
     good = dict(q=0x5000, stride=256, out=0x6000, heads=4, scale=0.125, window=0, sinks=0)
     for bad in (dict(q=0x5002), dict(q=None), dict(out=0x6008), dict(stride=248), dict(stride=260), dict(heads=3),
-                dict(heads=0), dict(scale=float("nan")), dict(scale=float("inf")), dict(window=-1), dict(sinks=-2)):
+                dict(heads=0), dict(heads=65538, stride=65538 * 64), dict(scale=float("nan")), dict(scale=float("inf")), dict(window=-1), dict(sinks=-2)):
         assert lib.ppocr_b200_kv4_attention(c, *(good | bad).values(), *p, 0x10000, None) == -1, bad
     for workspace in (None, 0x10080):
         assert lib.ppocr_b200_kv4_attention(c, *good.values(), *p, workspace, None) == -1

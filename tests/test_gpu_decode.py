@@ -472,6 +472,30 @@ def test_attention_on_a_side_stream_and_reused_workspace(native, cuda):
         assert torch.equal(x, first[0]) and torch.equal(y, first[1])
 
 
+def test_attention_of_thousands_of_sequences(native, cuda):
+    """More (sequence, row group) entries than one launch's prefix holds."""
+    lengths = [1 + (i * 7) % 40 for i in range(2600)]
+    s = Scene(lengths, [1] * 2600, 1, 32, 16, F16, seed=33, width=3)
+    s.fill(lengths)
+    cache = s.cache()
+    q = torch.randn(2600, 2, 32, generator=gen(34)).half()
+    got = cache.attention(q.cuda(), *s.places()).cpu().double()
+    assert fault(native) == 0
+    for b in (0, 1, 1023, 2047, 2048, 2049, 2599):
+        k, v = (O.held(s.pool, 16, 32, F16, s.table[b], lengths[b], w) for w in (0, 1))
+        want, mag, most = O.attention(q[b:b + 1], k, v, lengths[b] - 1, 32 ** -0.5)
+        tol = mag * (3.2 * U[F16] + torch.expm1(2.2 * 2.0 ** -20 * most)[..., None]) + 2.0 ** -24
+        assert ((got[b:b + 1] - want).abs() <= tol).all(), b
+
+
+@pytest.mark.parametrize("new,length,heads,kv", [(40, 6000, 2, 1), (130, 3000, 4, 2), (33, 2047, 1, 1)])
+def test_attention_prompt_over_a_long_cache(native, cuda, new, length, heads, kv):
+    """Few row blocks: several CTAs share a block's key tiles."""
+    s = Scene([length], [new], kv, 64, 64, F16, seed=length)
+    check_attention(native, s, heads, keys_rounded=True, rows={0, 1, 31, 39, 64, 128})
+    check_attention(native, s, heads, keys_rounded=True, window=900, sinks=3, rows={0, 39})
+
+
 def test_append_then_attention_then_append(native, cuda):
     """Token by token through the cache equals the whole prompt at once."""
     s = Scene([70], [70], 2, 64, 16, F16, seed=30)
@@ -661,6 +685,15 @@ def test_sample_flat_distributions(native, cuda, vocab, kw):
     x[3, : vocab // 2] = -math.inf
     check_sample(x, u, **kw)
     assert fault(native) == 0
+
+
+def test_sample_many_rows(native, cuda):
+    """More rows than a grid's second dimension holds."""
+    x = torch.zeros(70000, 24)
+    at = torch.arange(70000) % 24
+    x[torch.arange(70000), at] = 30.0
+    ids, _, kept = draw(x, torch.full((70000,), 0.5), top_p=0.9)
+    assert torch.equal(ids, at) and (kept == 1).all()
 
 
 def test_sample_frequencies(native, cuda):
