@@ -219,20 +219,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     *abort = 0;
     fence_barrier_init();
   }
-  // All of TMEM is taken only after the kernels before have ended, and the
-  // next kernel is let in only after it is taken: neither side can hold
-  // columns that the other's unfinished CTAs wait for.
   pdl_wait();
-  if (warp == 0) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  pdl_launch_dependents();
-  const uint32_t tmem = *tmem_slot;
-
   // Last rows first: they see the most keys.
   const uint32_t place = g.split_div.div(blockIdx.x);
   const int split = blockIdx.x - place * g.splits;
@@ -264,13 +251,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
   const int parts = share ? (tiles + share - 1) / share : 0, tile0 = split * share;
   tiles = min(max(tiles - tile0, 0), share);
   const bool two = rows > 128;
+  if (tiles == 0) // nothing of this block in this sequence
+    return;
+
+  // All of TMEM is taken only after the kernels before have ended, and the
+  // next kernel is let in only after it is taken: neither side can hold
+  // columns that the other's unfinished CTAs wait for.
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  const uint32_t tmem = *tmem_slot;
+
   auto key_of_tile = [&](int j) {
     j += tile0;
     return (j < sink ? j : j - sink + lo) * kTile;
   };
   bool ok = true;
 
-  if (tiles > 0 && warp < 8) {
+  if (warp < 8) {
     // ------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int block = warp >> 2;
@@ -542,7 +545,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         }
       }
     }
-  } else if (tiles > 0) {
+  } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp < 8 + kRestoreWarps) {
       // ----------------------------------------------------------- restoring
