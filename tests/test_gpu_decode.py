@@ -687,6 +687,15 @@ def test_sample_flat_distributions(native, cuda, vocab, kw):
     assert fault(native) == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, F16, BF16])
+@pytest.mark.parametrize("kw", [{}, {"top_k": 60, "top_p": 0.9, "temperature": 0.7}, {"top_p": 0.8, "min_p": 0.001},
+                                {"temperature": 0.0}])
+def test_sample_rows_longer_than_a_cluster_holds(native, cuda, dtype, kw):
+    x, u = logits_of(2, 500001, 91, dtype)
+    check_sample(x, u, **kw)
+    assert fault(native) == 0
+
+
 def test_sample_many_rows(native, cuda):
     """More rows than a grid's second dimension holds."""
     x = torch.zeros(70000, 24)
