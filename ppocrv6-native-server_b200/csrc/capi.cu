@@ -96,8 +96,8 @@ const char *kv4_arguments(const PpocrKv4Cache *cache, const int *table, int widt
   if (cache->kv_heads <= 0 || cache->kv_heads > 4096 || cache->pages <= 0 ||
       cache->pages > ((1ll << 31) - 1) / cache->kv_heads)
     return "kv_heads must be 1 to 4096, pages positive, pages * kv_heads below 2^31";
-  if (batch < 0 || batch > 65535 || tokens < 0 || max_new < 0)
-    return "batch (at most 65535), tokens and max_new must not be negative";
+  if (batch < 0 || batch > 65535 || tokens < 0 || max_new < 0 || max_new >= 1 << 30)
+    return "batch (at most 65535), tokens and max_new (below 2^30) must not be negative";
   if (!table || !lengths || width <= 0 || width >= (1 << 30) / cache->page_size)
     return "table or lengths missing, or table width out of range";
   if (!starts && static_cast<long long>(batch) * max_new != tokens)
@@ -120,13 +120,6 @@ const char *kv4_arguments(const PpocrKv4Cache *cache, const int *table, int widt
     ++t.page_shift;
   t.err = device_error_word();
   return nullptr;
-}
-// New tokens of one sequence, in 8-channel chunks of all keys and values, are
-// counted in 31 bits.
-const char *kv4_row_arguments(const PpocrKv4Cache *cache, int max_new) {
-  return static_cast<long long>(max_new) * cache->kv_heads * (cache->head_dim / 4) >= (1ll << 31) - (1 << 12)
-             ? "max_new * kv_heads * head_dim is too large"
-             : nullptr;
 }
 } // namespace
 
@@ -770,8 +763,6 @@ int ppocr_b200_kv4_append(const PpocrKv4Cache *cache, const void *k, long long k
     Kv4Cache c;
     Kv4Tokens t;
     const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
-    if (!bad)
-      bad = kv4_row_arguments(cache, max_new);
     if (bad)
       return fail(std::string("kv4 append: ") + bad);
     if (batch == 0 || tokens == 0 || max_new == 0)
@@ -791,8 +782,6 @@ int ppocr_b200_kv4_read(const PpocrKv4Cache *cache, void *k, void *v, const int 
     Kv4Cache c;
     Kv4Tokens t;
     const char *bad = kv4_arguments(cache, table, width, lengths, starts, batch, tokens, max_new, c, t);
-    if (!bad)
-      bad = kv4_row_arguments(cache, max_new);
     if (bad)
       return fail(std::string("kv4 read: ") + bad);
     if (batch == 0 || tokens == 0 || max_new == 0)

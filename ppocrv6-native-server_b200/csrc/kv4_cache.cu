@@ -5,18 +5,22 @@
 //  * append: a thread owns a group of 32 channels: four 16-byte loads, packed
 //    16-bit minimum and maximum, one reciprocal per group, a 16-byte store of
 //    codes and a 4-byte one of (scale, minimum). Next to the bytes it is close
-//    to being bound by its instructions (about nine a value): with a thread on
-//    eight channels, which repeats the group's work four times, it took 212 us
-//    where it now takes 65. Values that are not finite or beyond the limit are
-//    looked for in the bit patterns and put right on a path of their own.
+//    to being bound by its instructions (a thread on eight channels, which
+//    repeats the group's work four times, took 212 us where this takes 67).
+//    Values that are not finite or beyond the limit are looked for in the bit
+//    patterns and put right on a path of their own.
 //  * read: a thread owns eight channels of a key and of its value, so that
 //    its 16-byte stores and its neighbours' are whole lines, and takes four
-//    such items, all loads before the first use (two: 82 us, four: 75).
+//    such items, all loads before the first use (two: 82 us, four: 75, and 66
+//    since the places below are computed once).
 // Measured on 61,337 tokens of 8 heads of 128 (bf16, 330 MB moved): append
-// 65 us, 5.0 TB/s; read 75 us, 4.4 TB/s.
-// Blocks are laid out over (items of a sequence) x (sequence): ragged batches
-// leave blocks that only exit.
+// 67 us, 4.9 TB/s; read 66 us, 5.0 TB/s.
+// A thread keeps its place within a token (operand, head, part) and moves over
+// tokens, so that what it computes per item is one table lookup and an address.
+// Blocks are laid out over (tokens of a sequence) x (sequence) x (places past
+// a block's threads): ragged batches leave blocks that only exit.
 #include "kv4.cuh"
+#include <algorithm>
 
 namespace pb2 {
 namespace {
@@ -31,41 +35,30 @@ struct CacheArgs {
   uint16_t *ko, *vo;     // read: destination rows
   long long k_stride, v_stride;
   int kv_heads;
-  FastDiv token_div; // by the items of one token
+  int of_token;  // items of one token
+  int per_block; // tokens a block works on at once
+  FastDiv token_div; // by of_token
 };
 
-// Where an item sits: `per` items to a head; with BOTH, all of a token's key
-// items come before its value items.
-struct Spot {
-  bool live;      // of a token of this sequence
-  bool held;      // with a position in the cache
-  bool value;     // of the values, not the keys
-  int head, part; // part of the head
-  long long row;  // packed row
-  uint8_t *block; // (page, head) block
-  int slot;       // token within the page
+// A thread's place: item `in` of every token it meets, the first of them, and
+// how far the next is.
+struct Place {
+  int in, tok, step;
+  bool live;
 };
-template <int D, bool BOTH>
-__device__ __forceinline__ Spot spot_of(const CacheArgs &g, const Kv4Seq &q, uint32_t item, int per) {
-  Spot s;
-  const uint32_t tok = g.token_div.div(item);
-  const int in = item - tok * ((BOTH ? 2 : 1) * g.kv_heads * per);
-  s.value = BOTH && in >= g.kv_heads * per;
-  const int at = in - (s.value ? g.kv_heads * per : 0);
-  s.head = at / per; // a power of two
-  s.part = at % per;
-  s.live = tok < static_cast<uint32_t>(q.n);
-  const int pos = q.len - q.n + static_cast<int>(tok);
-  s.held = s.live && pos >= 0;
-  s.row = q.first + static_cast<long long>(tok);
-  s.block = nullptr;
-  s.slot = 0;
-  if (s.held) {
-    const long long page = kv4_page(g.t, blockIdx.y, pos);
-    s.slot = pos & ((1 << g.t.page_shift) - 1);
-    s.block = g.pool + (page * g.kv_heads + s.head) * static_cast<long long>((D + D / 4) << g.t.page_shift);
-  }
-  return s;
+__device__ __forceinline__ Place place_of(const CacheArgs &g, int items) {
+  Place p;
+  const int local = g.of_token <= kThreads ? g.token_div.div(threadIdx.x) : 0;
+  p.in = blockIdx.z * kThreads + threadIdx.x - local * g.of_token;
+  p.tok = blockIdx.x * g.per_block * items + local;
+  p.step = g.per_block;
+  p.live = p.in < g.of_token;
+  return p;
+}
+// The (page, head) block of a position.
+template <int D> __device__ __forceinline__ uint8_t *block_of(const CacheArgs &g, int head, int pos) {
+  const long long page = kv4_page(g.t, blockIdx.y, pos);
+  return g.pool + (page * g.kv_heads + head) * static_cast<long long>((D + D / 4) << g.t.page_shift);
 }
 
 template <bool BF16> struct Packed;
@@ -104,6 +97,11 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  ffma2(c, a, b);
+  return c;
 }
 
 // Quantises a group of 32 channels (16 words): its codes and its (scale,
@@ -161,19 +159,25 @@ template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ CacheArgs g) {
   pdl_begin();
   const Kv4Seq q = kv4_seq(g.t, blockIdx.y);
-  const Spot s = spot_of<D, true>(g, q, blockIdx.x * kThreads + threadIdx.x, D / 32);
-  if (!s.held)
+  const Place at = place_of(g, 1);
+  const int pos = q.len - q.n + at.tok;
+  if (!at.live || at.tok >= q.n || pos < 0)
     return;
-  const uint16_t *src = (s.value ? g.v + s.row * g.v_stride : g.k + s.row * g.k_stride) + s.head * D + s.part * 32;
+  const int of_keys = g.of_token / 2;
+  const bool value = at.in >= of_keys;
+  const int in = at.in - (value ? of_keys : 0), head = in / (D / 32), part = in % (D / 32);
+  const long long row = q.first + static_cast<long long>(at.tok);
+  const uint16_t *src = (value ? g.v + row * g.v_stride : g.k + row * g.k_stride) + in * 32;
+  uint8_t *block = block_of<D>(g, head, pos);
+  const int page = 1 << g.t.page_shift, slot = (pos & (page - 1)) + (value ? page : 0);
   uint4 x[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     x[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
   uint32_t params;
   const uint4 codes = quantise<BF16>(x, params);
-  const int page = 1 << g.t.page_shift, slot = s.slot + (s.value ? page : 0);
-  *reinterpret_cast<uint4 *>(s.block + slot * (D / 2) + s.part * 16) = codes;
-  *reinterpret_cast<uint32_t *>(s.block + page * D + slot * (D / 8) + s.part * 4) = params;
+  *reinterpret_cast<uint4 *>(block + slot * (D / 2) + part * 16) = codes;
+  *reinterpret_cast<uint32_t *>(block + page * D + slot * (D / 8) + part * 4) = params;
 }
 
 template <bool BF16> __device__ __forceinline__ uint4 restore8(uint32_t codes, uint32_t params) {
@@ -185,7 +189,7 @@ template <bool BF16> __device__ __forceinline__ uint4 restore8(uint32_t codes, u
     const float2 c = add2(make_float2(__uint_as_float(0x4B000000u | ((codes >> (8 * i)) & 15u)),
                                       __uint_as_float(0x4B000000u | ((codes >> (8 * i + 4)) & 15u))),
                           make_float2(-8388608.f, -8388608.f));
-    const float2 x = add2(mul2(c, make_float2(scale, scale)), make_float2(lo, lo));
+    const float2 x = fma2(c, make_float2(scale, scale), make_float2(lo, lo));
     w[i] = kv4_pack<BF16>(x.x, x.y);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
@@ -195,46 +199,51 @@ template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ CacheArgs g) {
   pdl_begin();
   const Kv4Seq q = kv4_seq(g.t, blockIdx.y);
-  const uint32_t item0 = blockIdx.x * (kThreads * kReadItems) + threadIdx.x;
+  const Place at = place_of(g, kReadItems);
+  if (!at.live || at.tok >= q.n)
+    return;
+  const int head = at.in / (D / 8), part = at.in % (D / 8);
   const int page = 1 << g.t.page_shift;
-  Spot s[kReadItems];
   uint32_t codes[kReadItems][2], params[kReadItems][2];
 #pragma unroll
   for (int n = 0; n < kReadItems; ++n) {
-    s[n] = spot_of<D, false>(g, q, item0 + n * kThreads, D / 8);
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      codes[n][v] = params[n][v] = 0; // without a position: zeros
-      if (s[n].held) {
-        const int slot = s[n].slot + (v ? page : 0);
-        codes[n][v] = __ldg(reinterpret_cast<const uint32_t *>(s[n].block + slot * (D / 2) + s[n].part * 4));
-        params[n][v] =
-            __ldg(reinterpret_cast<const uint32_t *>(s[n].block + page * D + slot * (D / 8) + s[n].part / 4 * 4));
-      }
+    const int tok = at.tok + n * at.step, pos = q.len - q.n + tok;
+    codes[n][0] = codes[n][1] = params[n][0] = params[n][1] = 0; // without a position: zeros
+    if (tok < q.n && pos >= 0) {
+      const int slot = pos & (page - 1);
+      const uint8_t *block = block_of<D>(g, head, pos);
+      const uint8_t *c = block + slot * (D / 2) + part * 4, *p = block + page * D + slot * (D / 8) + part / 4 * 4;
+      codes[n][0] = __ldg(reinterpret_cast<const uint32_t *>(c));
+      codes[n][1] = __ldg(reinterpret_cast<const uint32_t *>(c + page * (D / 2)));
+      params[n][0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+      params[n][1] = __ldg(reinterpret_cast<const uint32_t *>(p + page * (D / 8)));
     }
   }
 #pragma unroll
-  for (int n = 0; n < kReadItems; ++n)
-    if (s[n].live) {
-      const long long e = (s[n].row * g.kv_heads + s[n].head) * D + s[n].part * 8;
-      *reinterpret_cast<uint4 *>(g.ko + e) = restore8<BF16>(codes[n][0], params[n][0]);
-      *reinterpret_cast<uint4 *>(g.vo + e) = restore8<BF16>(codes[n][1], params[n][1]);
-    }
+  for (int n = 0; n < kReadItems; ++n) {
+    const int tok = at.tok + n * at.step;
+    if (tok >= q.n)
+      break;
+    const long long e = ((q.first + static_cast<long long>(tok)) * g.of_token + at.in) * 8;
+    *reinterpret_cast<uint4 *>(g.ko + e) = restore8<BF16>(codes[n][0], params[n][0]);
+    *reinterpret_cast<uint4 *>(g.vo + e) = restore8<BF16>(codes[n][1], params[n][1]);
+  }
 }
 
 template <int D, bool BF16> cudaError_t launch(CacheArgs g, bool append, cudaStream_t s) {
-  const int of_token = g.kv_heads * (append ? 2 * D / 32 : D / 8);
-  const int per_block = kThreads * (append ? 1 : kReadItems);
-  g.token_div = FastDiv(of_token);
-  const long long items = static_cast<long long>(g.t.max_new) * of_token;
-  const dim3 grid(static_cast<unsigned>((items + per_block - 1) / per_block), g.t.batch);
-  return launch_pdl(append ? append_kernel<D, BF16> : read_kernel<D, BF16>, grid, kThreads, 0, s, g);
+  const int items = append ? 1 : kReadItems;
+  g.of_token = g.kv_heads * (append ? 2 * D / 32 : D / 8);
+  g.token_div = FastDiv(g.of_token);
+  g.per_block = std::max(1, std::min(kThreads / g.of_token, (g.t.max_new + items - 1) / items));
+  const int tokens = g.per_block * items;
+  const dim3 grid(static_cast<unsigned>((static_cast<long long>(g.t.max_new) + tokens - 1) / tokens), g.t.batch,
+                  (g.of_token + kThreads - 1) / kThreads);
+  const int threads = g.of_token <= kThreads ? g.per_block * g.of_token : kThreads;
+  return launch_pdl(append ? append_kernel<D, BF16> : read_kernel<D, BF16>, grid, threads, 0, s, g);
 }
 
 cudaError_t dispatch(const Kv4Cache &c, const CacheArgs &g, bool append, cudaStream_t s) {
-  // Items of a sequence's new tokens are counted in 31 bits.
-  if (static_cast<long long>(g.t.max_new) * c.kv_heads * (c.head_dim / 4) >= (1ll << 31) - (1 << 12) ||
-      g.t.batch > 65535)
+  if (g.t.batch > 65535)
     return cudaErrorInvalidValue;
   switch (c.head_dim * 2 + c.bf16) {
   case 64: return launch<32, false>(g, append, s);

@@ -24,9 +24,14 @@
 //  5. the draw: a scan of the threads' kept masses, in index order.
 // Rows longer than a cluster's shared memory take the digit search alone.
 // Bound by the instructions of step 1 (a division, an exponential and a 64-bit
-// sum per logit); the steps after it touch only what passes a comparison,
-// each lane working off its own hits (a mask of 32 logits a lane) so that few
-// hits cost few turns of the warp.
+// sum per logit: issue slots 66 % busy, ALU 52 %) and, for few rows, by the
+// cluster's exchanges (about half a microsecond each); the steps after it touch
+// only what passes a comparison, each lane working off its own hits (a mask of
+// 32 logits a lane) so that few hits cost few turns of the warp.
+// Measured: 96 rows of 131,072 bf16 logits, p 0.98 and min-p 0.01: 58 us, 431
+// GB/s; 256 rows of 18,385 fp32 logits, p 0.9: 33 us; 4 rows of 18,385, k 50
+// and p 0.95: 21 us; greedy 9 us. The digit search alone (four passes over the
+// row per bound) took 5.6 ms, 0.5 ms and 0.5 ms for the first three.
 #include "kernels.h"
 #include "ptx.cuh"
 #include <algorithm>
