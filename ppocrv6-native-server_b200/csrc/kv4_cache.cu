@@ -11,8 +11,8 @@
 //    patterns and put right on a path of their own.
 //  * read: a thread owns eight channels of a key and of its value, so that
 //    its 16-byte stores and its neighbours' are whole lines, and takes four
-//    such items, all loads before the first use (two: 82 us, four: 75, and 66
-//    since the places below are computed once).
+//    such items, all loads before the first use (two 82 us, three 76, four
+//    75, before the places below were computed once: 66.5 since).
 // Measured on 61,337 tokens of 8 heads of 128 (bf16, 330 MB moved): append
 // 67 us, 4.9 TB/s; read 66 us, 5.0 TB/s.
 // A thread keeps its place within a token (operand, head, part) and moves over

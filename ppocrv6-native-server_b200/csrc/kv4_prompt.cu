@@ -29,15 +29,17 @@
 // of one: each leaves (m, l, O) of its rows in fp32, and per 32 rows the last
 // warp to arrive joins them in the order of the tiles.
 // Work per tile: 4 x 128 x 128 x D multiply-adds (2048 cycles of the tensor
-// pipe at D = 128, 2280 measured for the four products alone) against 32768
-// exponentials (2048 cycles of the special function units). Measured, a tile
-// takes about 4400 cycles: a row's softmax (load, maximum, powers: 2600) and
-// its block's two products follow one another, and the restoring warps share
-// the ALU pipe with it (43 % busy). 2 sequences of 4096 tokens, 16 heads of
-// 128 on 4 key heads, causal: bf16 184 us, 747 TFLOP/s (fp16 about 170); chunks
-// of 507 tokens over 7,250 through a window of 4096, 4 sequences, fp16: 92 us,
-// 740 TFLOP/s; 48 ragged prompts of 160 tokens, 8 heads of 64: 34 us, three
-// waves of CTAs bound by their own latency.
+// pipe at D = 128) against 32768 exponentials (2048 cycles of the special
+// function units). Neither is busy all the time (ncu, first size below: tensor
+// pipe 32 %, special functions 32 %, ALU 42 %, issue slots 49 %): a block's
+// scores, softmax and product follow one another. Clock counters in an
+// instrumented copy of an earlier build (192 us) gave per tile 1780 cycles of
+// waiting for scores, 110 loading them, 690 for masks and maximum, 1880 for
+// powers and sums. Measured: 2 sequences of 4096 tokens, 16 heads of 128 on 4
+// key heads, causal: bf16 190 us, 724 TFLOP/s, fp16 167 us; chunks of 500 to
+// 513 tokens over 7,000 to 7,500 through a window of 4096, 4 sequences, fp16:
+// 92 us, 740 TFLOP/s; 48 prompts of 21 to 300 tokens, 8 heads of 64, fp16: 34.6
+// us (one CTA an SM, so a prompt's CTAs run in about three rounds).
 #include "kv4.cuh"
 #include <algorithm>
 #include <cmath>

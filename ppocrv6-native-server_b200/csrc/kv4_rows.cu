@@ -36,13 +36,14 @@
 // large as it is, so that it stays below 2^14 and fp16 holds what is 2^-30 of
 // the largest.
 //
-// Bound by instructions: about 400 a warp for 16 keys at D = 128, mostly masks
-// and conversions of codes (ncu at the first size below: issue slots 65 % busy,
-// ALU 59 %, DRAM 50 %, tensor pipe 20 %). Three CTAs of five warps an SM;
+// Bound by instructions: 407 warp instructions per 16 keys of a key head at
+// D = 128, everything counted (ncu at the first size below: issue slots 65 %
+// busy, ALU 59 %, DRAM 50 %, tensor pipe 20 %). Three CTAs of five warps an SM;
 // measured, fp16, 16 sequences of 32,384 keys in 8 heads of 128, 32 query heads:
 // 155 us, 4.3 TB/s of 663 MB; bf16, 64 sequences of 1,090 keys on average in 4
 // heads of 128, 16 query heads: 28 us, of which the scan of the lengths, the
-// queries' loading, merging and joining take a third.
+// queries' loading, merging and joining take about 30 % (clock counters in an
+// instrumented copy).
 //
 // Keys past a sequence's length are never used: their scores are replaced
 // (not multiplied) and their values' parameters zeroed, so a page may hold

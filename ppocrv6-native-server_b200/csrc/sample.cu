@@ -23,15 +23,17 @@
 //     is resolved digit by digit of the key instead, over the row in memory;
 //  5. the draw: a scan of the threads' kept masses, in index order.
 // Rows longer than a cluster's shared memory take the digit search alone.
-// Bound by the instructions of step 1 (a division, an exponential and a 64-bit
-// sum per logit: issue slots 66 % busy, ALU 52 %) and, for few rows, by the
-// cluster's exchanges (about half a microsecond each); the steps after it touch
-// only what passes a comparison, each lane working off its own hits (a mask of
-// 32 logits a lane) so that few hits cost few turns of the warp.
-// Measured: 96 rows of 131,072 bf16 logits, p 0.98 and min-p 0.01: 58 us, 431
+// At many logits bound by the instructions of step 1 (a division, an
+// exponential and a 64-bit sum per logit; ncu, first size below: issue slots
+// 66 % busy, ALU 52 %, DRAM 4 %); the steps after it touch only what passes a
+// comparison, each lane working off its own hits (a mask of 32 logits a lane)
+// so that few hits cost few turns of the warp. Few rows are bound by the chain
+// of steps and cluster exchanges.
+// Measured: 96 rows of 131,072 bf16 logits, p 0.98 and min-p 0.01: 59 us, 430
 // GB/s; 256 rows of 18,385 fp32 logits, p 0.9: 33 us; 4 rows of 18,385, k 50
-// and p 0.95: 21 us; greedy 9 us. The digit search alone (four passes over the
-// row per bound) took 5.6 ms, 0.5 ms and 0.5 ms for the first three.
+// and p 0.95: 21 us; k 1 or temperature 0: 8 us for 4 rows of 18,385 fp32, 19
+// us for 256. The digit search alone took 5.6 ms, 0.50 ms and 0.52 ms a call
+// for the first three.
 #include "kernels.h"
 #include "ptx.cuh"
 #include <algorithm>
